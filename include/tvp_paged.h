@@ -398,6 +398,113 @@ int tvp_head_gather_disconnect(tvp_head_gather* g);
 int tvp_head_gather_destroy(tvp_head_gather* g);
 
 /* ======================================================================= *
+ * Attention over part of a row's pages, and over pages that rows share.  No
+ * counterparts in the reference, whose decode attends each row's whole
+ * context on its own (src/model/paged_transformer.cu:85-94).  Pools, tables
+ * and error bits are as above; kv_heads is 8, 4, 2 or 1, q_heads = 4 kv_heads.
+ * Scores and softmax statistics are FP32, probabilities BF16 into an FP32
+ * P.V, outputs BF16.
+ * ======================================================================= */
+
+/*
+ * Workspace of the two decode entry points below, for up to `batch` rows and
+ * `groups` prefix groups (0: window decode only) on `num_ctas` CTAs (0 = one
+ * per SM).  256-byte aligned, a multiple of 4 bytes in size, zeroed once
+ * before its first use: every launch leaves its arrival counters zero.  One
+ * workspace serves calls of any batch, groups and kv_heads that fit it; calls
+ * that share it must not overlap on the GPU, and after a TVP_DEVERR_TIMEOUT it
+ * must be zeroed again.  0 for arguments out of range.
+ */
+size_t tvp_span_workspace_bytes(int batch, int groups, int kv_heads, int num_ctas);
+
+/*
+ * K6 — decode attention with a sliding window and attention sinks.
+ * Row b's query is its last token, at position L - 1 (L = d_seq_lens[b]); it
+ * attends the last `window` tokens, itself among them, and the first `sinks`
+ * tokens: key j < L is visible when j >= L - window or j < sinks.  window >= 1,
+ * sinks >= 0; a row with L <= 0 gets zeros (negative: TVP_DEVERR_BAD_LENGTH).
+ * Pages without a visible token are not read: their table entries may be
+ * anything (-1 once the page was given back), and hidden tokens of pages that
+ * are read may hold NaN.  No plan is needed: d_seq_lens is read by the kernel.
+ * As tvp_paged_decode_attention, the launch is a programmatic dependent one:
+ * a kernel that releases its dependents early must not write d_seq_lens or the
+ * block tables when it runs right before this call.
+ */
+int tvp_paged_window_decode_attention(const tvp_bf16* q, const tvp_bf16* k_pool,
+                                      const tvp_bf16* v_pool, int num_pages, int num_layers,
+                                      int layer, int kv_heads, int q_heads,
+                                      const int32_t* d_block_tables, int table_stride,
+                                      const int32_t* d_seq_lens, int batch, int window, int sinks,
+                                      float scale, int num_ctas, void* d_workspace,
+                                      size_t workspace_bytes, tvp_bf16* out, int32_t* d_error,
+                                      tvp_stream_t stream);
+
+/*
+ * K7 — decode attention of a batch whose rows share long prefixes, each prefix
+ * read once per 32 rows of its group instead of once per row.
+ * Group g holds the rows [d_group_rows[g], d_group_rows[g + 1]) (non-decreasing,
+ * within 0..batch; rows outside every group share nothing).  The first
+ * 16 * d_prefix_pages[g] tokens of each of its rows are the pages
+ * d_prefix_tables[g * prefix_stride ..]; a row's later tokens are on the pages
+ * of its own block-table row, which stays indexed by position (entry
+ * position / 16; the entries of the shared pages are not read).  Row b attends
+ * its first d_seq_lens[b] tokens.  A row of length 0 gets zeros; one shorter
+ * than its prefix gets zeros and TVP_DEVERR_BAD_LENGTH.  Group rows that are
+ * out of order set TVP_DEVERR_BAD_PLAN and nothing is written.  groups = 0 is
+ * plain decode attention.  Two launches on `stream`; what a call right before
+ * may write while it releases its dependents early is as for K6.
+ */
+int tvp_paged_shared_prefix_decode_attention(
+    const tvp_bf16* q, const tvp_bf16* k_pool, const tvp_bf16* v_pool, int num_pages,
+    int num_layers, int layer, int kv_heads, int q_heads, const int32_t* d_block_tables,
+    int table_stride, const int32_t* d_seq_lens, int batch, const int32_t* d_prefix_tables,
+    int prefix_stride, const int32_t* d_prefix_pages, const int32_t* d_group_rows, int groups,
+    float scale, int num_ctas, void* d_workspace, size_t workspace_bytes, tvp_bf16* out,
+    int32_t* d_error, tvp_stream_t stream);
+
+/*
+ * K8 — causal prefill attention with a sliding window and attention sinks,
+ * over the pages: tvp_paged_prefill_attention's queries and layout, where the
+ * query at position p sees key j <= p when j > p - window or j < sinks.  Pages
+ * that no query of a 32-token tile sees are not read by that tile.
+ */
+int tvp_paged_window_prefill_attention(const tvp_bf16* q, const tvp_bf16* k_pool,
+                                       const tvp_bf16* v_pool, int num_pages, int num_layers,
+                                       int layer, int kv_heads, int q_heads,
+                                       const int32_t* d_block_tables, int table_stride,
+                                       const int32_t* d_cu_q, const int32_t* d_q_pos0,
+                                       int num_seqs, int max_q_len, int window, int sinks,
+                                       float scale, tvp_bf16* out, int32_t* d_error,
+                                       tvp_stream_t stream);
+
+/*
+ * K9 — draws one token per row of FP32 logits from given random numbers.
+ * Row r, with x the logits (NaN counts as -inf), T = d_temperature[r] and
+ * w_i = exp((x_i - max x) / T):
+ *   1. top-k: the d_top_k[r] largest logits stay, ties to the lowest index
+ *      (<= 0: all);
+ *   2. top-p: of these, in falling order (ties by index), the shortest run
+ *      whose w sum to at least d_top_p[r] of theirs, at least one (>= 1: all);
+ *   3. min-p: of these, the ones with w_i >= min(d_min_p[r], 1) (<= 0: all);
+ *   4. the token is the first one left, in index order, where the running sum
+ *      of w exceeds d_uniforms[r] times the whole sum; uniforms are in [0, 1)
+ *      (values outside are taken as the nearest end).
+ * T <= 0 takes the largest logit (lowest index).  A row without any logit
+ * above -inf gives token -1; +inf logits share the whole mass.  d_temperature,
+ * d_top_k, d_top_p and d_min_p may each be null: 1, off, off, off; a NaN
+ * setting is off (a NaN temperature: the largest logit).  Weights are summed
+ * as 64-bit integers of 2^-44 of the largest weight, so the result does not
+ * depend on the order of the sums.  Unlike tvp_greedy_argmax, logits are not
+ * rounded to BF16.  d_logits: [rows][row_stride], row_stride >= vocab; vocab at
+ * most TVP_SAMPLE_MAX_VOCAB.  No workspace.
+ */
+#define TVP_SAMPLE_MAX_VOCAB 393216
+int tvp_sample_tokens(const float* d_logits, int rows, int vocab, long long row_stride,
+                      const float* d_uniforms, const float* d_temperature, const int32_t* d_top_k,
+                      const float* d_top_p, const float* d_min_p, int32_t* d_tokens,
+                      tvp_stream_t stream);
+
+/* ======================================================================= *
  * Host API mirror: PagedKVCache / SequenceKVState / PagedBatchMetadata.
  * Same allocator semantics as src/model/paged_kvcache.cu:37-117 (LIFO free
  * list seeded descending, lazy ceil(L/16) pages, exhaustion checked before

@@ -88,6 +88,23 @@ _SIGNATURES = {
                                          c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                                          c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "tvp_span_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "tvp_paged_window_decode_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                                  c_int, c_int, c_int, c_void_p, c_int, c_void_p,
+                                                  c_int, c_int, c_int, c_float, c_int, c_void_p,
+                                                  c_size_t, c_void_p, c_void_p, c_void_p]),
+    "tvp_paged_shared_prefix_decode_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_int,
+                                                         c_int, c_int, c_int, c_int, c_void_p,
+                                                         c_int, c_void_p, c_int, c_void_p, c_int,
+                                                         c_void_p, c_void_p, c_int, c_float,
+                                                         c_int, c_void_p, c_size_t, c_void_p,
+                                                         c_void_p, c_void_p]),
+    "tvp_paged_window_prefill_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                                   c_int, c_int, c_int, c_void_p, c_int, c_void_p,
+                                                   c_void_p, c_int, c_int, c_int, c_int, c_float,
+                                                   c_void_p, c_void_p, c_void_p]),
+    "tvp_sample_tokens": (c_int, [c_void_p, c_int, c_int, ctypes.c_longlong, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "tvp_head_gather_create": (c_int, [c_int, c_int, c_int, c_int, POINTER(c_void_p)]),
     "tvp_head_gather_export": (c_int, [c_void_p, c_void_p]),
     "tvp_head_gather_connect": (c_int, [c_void_p, c_void_p]),

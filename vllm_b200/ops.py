@@ -232,6 +232,216 @@ def greedy_argmax(logits, out=None, workspace=None, stream=None):
     return out
 
 
+class SpanWorkspace:
+    """Device workspace of :func:`paged_window_decode_attention` and
+    :func:`paged_shared_prefix_decode_attention` for up to ``max_batch`` rows
+    and ``max_groups`` prefix groups of a pool of ``kv_heads`` KV heads, on
+    ``num_ctas`` CTAs (0 = one per SM).  Calls that share one must not overlap
+    on the GPU; :meth:`reset` makes it usable again after a launch timed out."""
+
+    def __init__(self, max_batch: int, device=None, num_ctas: int = 0, kv_heads: int = N.KV_HEADS,
+                 max_groups: int = 0):
+        lib = N.load()
+        device = torch.device(device if device is not None else "cuda")
+        with torch.cuda.device(device):
+            sms = ctypes.c_int(0)
+            N.check(lib.tvp_device_sm_count(ctypes.byref(sms)), "tvp_device_sm_count")
+            self.num_ctas = num_ctas if num_ctas > 0 else sms.value
+            self.nbytes = int(lib.tvp_span_workspace_bytes(max_batch, max_groups, kv_heads,
+                                                           self.num_ctas))
+            if self.nbytes == 0:
+                raise ValueError("invalid workspace request")
+            self.buffer = torch.zeros(self.nbytes, dtype=torch.uint8, device=device)
+        self.max_batch = max_batch
+        self.max_groups = max_groups
+        self.kv_heads = kv_heads
+
+    def reset(self):
+        self.buffer.zero_()
+
+
+def _on(dev, stream):
+    """The stream a call runs on: the given one, which must be of the tensors'
+    device, or that device's current one."""
+    if stream is None:
+        return torch.cuda.current_stream(dev)
+    if stream.device != dev:
+        raise ValueError(f"stream is of {stream.device}, the tensors are on {dev}")
+    return stream
+
+
+def _output(out, like, stream):
+    """``out``, or a tensor like ``like`` that belongs to the call's stream."""
+    if out is None:
+        with torch.cuda.stream(stream):
+            return torch.empty_like(like)
+    _need(out, "out", like.dtype, like.device)
+    if out.shape != like.shape:
+        raise ValueError(f"out must be {list(like.shape)}")
+    return out
+
+
+def _need_error(error, dev):
+    if error is not None:
+        _need(error, "error", torch.int32, dev)
+
+
+def _decode_rows(q, k_pool, v_pool, block_tables, seq_lens, workspace, error):
+    """Argument checks of the span decode calls; the pools' geometry."""
+    num_layers, num_pages, kv_heads = _pool_geometry(k_pool, v_pool)
+    dev = k_pool.device
+    _need(q, "q", torch.bfloat16, dev)
+    _need(block_tables, "block_tables", torch.int32, dev)
+    _need(seq_lens, "seq_lens", torch.int32, dev)
+    _need_error(error, dev)
+    batch = seq_lens.numel()
+    if q.shape != (batch, kv_heads * N.GQA_GROUP * N.HEAD_DIM):
+        raise ValueError("q must be [batch, 4*kv_heads*64]")
+    if block_tables.dim() != 2 or block_tables.shape[0] < batch:
+        raise ValueError("block_tables must be [>=batch, table_stride]")
+    if workspace is None or workspace.buffer.device != dev:
+        raise ValueError("a SpanWorkspace on the tensors' device is required")
+    if workspace.kv_heads != kv_heads:
+        raise ValueError(f"workspace was sized for {workspace.kv_heads} KV heads, pools hold {kv_heads}")
+    if batch > workspace.max_batch:
+        raise ValueError("batch larger than the workspace was sized for")
+    return num_layers, num_pages, kv_heads, batch
+
+
+def paged_window_decode_attention(q, k_pool, v_pool, layer, block_tables, seq_lens, window,
+                                  workspace, sinks=0, out=None, scale=0.125, error=None,
+                                  stream=None):
+    """K6: decode attention with a sliding window and sinks.  Row b's query (its
+    last token) attends the last ``window`` of its ``seq_lens[b]`` tokens and the
+    first ``sinks``; a row of length 0 gets zeros.  Pages without a visible token
+    are not read (their table entries may be -1).  No plan is needed."""
+    lib = N.load()
+    num_layers, num_pages, kv_heads, batch = _decode_rows(q, k_pool, v_pool, block_tables,
+                                                          seq_lens, workspace, error)
+    dev = k_pool.device
+    with torch.cuda.device(dev):
+        st = _on(dev, stream)
+        out = _output(out, q, st)
+        rc = lib.tvp_paged_window_decode_attention(
+            _ptr(q), _ptr(k_pool), _ptr(v_pool), num_pages, num_layers, layer, kv_heads,
+            kv_heads * N.GQA_GROUP, _ptr(block_tables), block_tables.shape[1], _ptr(seq_lens),
+            batch, int(window), int(sinks), float(scale), workspace.num_ctas,
+            _ptr(workspace.buffer), workspace.nbytes, _ptr(out), _ptr(error), _stream(st))
+    N.check(rc, "tvp_paged_window_decode_attention")
+    return out
+
+
+def paged_shared_prefix_decode_attention(q, k_pool, v_pool, layer, block_tables, seq_lens,
+                                         prefix_tables, prefix_pages, group_rows, workspace,
+                                         out=None, scale=0.125, error=None, stream=None):
+    """K7: decode attention of a batch whose rows share prefixes.  Group g is the
+    rows [group_rows[g], group_rows[g + 1]); the first 16 * prefix_pages[g] tokens
+    of each of them are on the pages prefix_tables[g], read once for the group
+    (per 32 of its rows) and merged with each row's own later pages, which stay
+    at their places (position / 16) in ``block_tables``.  prefix_tables: int32
+    [groups, stride]; prefix_pages: int32 [groups]; group_rows: int32 [groups + 1]."""
+    lib = N.load()
+    num_layers, num_pages, kv_heads, batch = _decode_rows(q, k_pool, v_pool, block_tables,
+                                                          seq_lens, workspace, error)
+    dev = k_pool.device
+    _need(prefix_tables, "prefix_tables", torch.int32, dev)
+    _need(prefix_pages, "prefix_pages", torch.int32, dev)
+    _need(group_rows, "group_rows", torch.int32, dev)
+    groups = prefix_pages.numel()
+    if group_rows.numel() != groups + 1:
+        raise ValueError("group_rows must have groups + 1 entries")
+    if prefix_tables.dim() != 2 or prefix_tables.shape[0] < groups:
+        raise ValueError("prefix_tables must be [>=groups, prefix_stride]")
+    if groups > workspace.max_groups:
+        raise ValueError("more groups than the workspace was sized for")
+    with torch.cuda.device(dev):
+        st = _on(dev, stream)
+        out = _output(out, q, st)
+        rc = lib.tvp_paged_shared_prefix_decode_attention(
+            _ptr(q), _ptr(k_pool), _ptr(v_pool), num_pages, num_layers, layer, kv_heads,
+            kv_heads * N.GQA_GROUP, _ptr(block_tables), block_tables.shape[1], _ptr(seq_lens),
+            batch, _ptr(prefix_tables), prefix_tables.shape[1], _ptr(prefix_pages),
+            _ptr(group_rows), groups, float(scale), workspace.num_ctas, _ptr(workspace.buffer),
+            workspace.nbytes, _ptr(out), _ptr(error), _stream(st))
+    N.check(rc, "tvp_paged_shared_prefix_decode_attention")
+    return out
+
+
+def paged_window_prefill_attention(q, k_pool, v_pool, layer, block_tables, cu_q, q_pos0, max_q_len,
+                                   window, sinks=0, out=None, scale=0.125, error=None, stream=None):
+    """K8: :func:`paged_prefill_attention`'s queries with a sliding window and
+    sinks: the query at position p sees key j <= p when j > p - window or
+    j < sinks."""
+    lib = N.load()
+    num_layers, num_pages, kv_heads = _pool_geometry(k_pool, v_pool)
+    dev = k_pool.device
+    _need(q, "q", torch.bfloat16, dev)
+    _need(block_tables, "block_tables", torch.int32, dev)
+    _need(cu_q, "cu_q", torch.int32, dev)
+    _need(q_pos0, "q_pos0", torch.int32, dev)
+    _need_error(error, dev)
+    num_seqs = q_pos0.numel()
+    if cu_q.numel() != num_seqs + 1:
+        raise ValueError("cu_q must have num_seqs + 1 entries")
+    if q.dim() != 2 or q.shape[1] != kv_heads * N.GQA_GROUP * N.HEAD_DIM:
+        raise ValueError("q must be [num_tokens, 4*kv_heads*64]")
+    if block_tables.dim() != 2 or block_tables.shape[0] < num_seqs:
+        raise ValueError("block_tables must be [>=num_seqs, table_stride]")
+    with torch.cuda.device(dev):
+        st = _on(dev, stream)
+        out = _output(out, q, st)
+        if q.shape[0] == 0:
+            return out
+        rc = lib.tvp_paged_window_prefill_attention(
+            _ptr(q), _ptr(k_pool), _ptr(v_pool), num_pages, num_layers, layer, kv_heads,
+            kv_heads * N.GQA_GROUP, _ptr(block_tables), block_tables.shape[1], _ptr(cu_q),
+            _ptr(q_pos0), num_seqs, int(max_q_len), int(window), int(sinks), float(scale),
+            _ptr(out), _ptr(error), _stream(st))
+    N.check(rc, "tvp_paged_window_prefill_attention")
+    return out
+
+
+def sample_tokens(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, out=None,
+                  stream=None):
+    """K9: one token per row of FP32 logits [rows, vocab] (rows may be strided:
+    logits.stride(1) must be 1), drawn by ``uniforms[r]`` in [0, 1) from
+    softmax(logits / temperature) after top-k, top-p and min-p, in that order
+    (see tvp_sample_tokens).  temperature, top_p, min_p: FP32 [rows]; top_k:
+    int32 [rows]; each may be None (1, off, off, off).  Temperature 0 takes the
+    largest logit.  Returns int32 [rows]; -1 for a row without a logit above -inf."""
+    lib = N.load()
+    if not (logits.is_cuda and logits.dtype == torch.float32):
+        raise ValueError("logits must be a CUDA float32 tensor")
+    if logits.dim() != 2 or logits.stride(1) != 1 or \
+            (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+        raise ValueError("logits must be [rows, vocab] with unit stride along vocab")
+    rows, vocab = logits.shape
+    dev = logits.device
+    _need(uniforms, "uniforms", torch.float32, dev)
+    per_row = [(uniforms, "uniforms")]
+    for t, name, dtype in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32),
+                           (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
+        if t is not None:
+            _need(t, name, dtype, dev)
+            per_row.append((t, name))
+    for t, name in per_row:
+        if t.numel() != rows:
+            raise ValueError(f"{name} must have one entry per row")
+    with torch.cuda.device(dev):
+        st = _on(dev, stream)
+        if out is None:
+            with torch.cuda.stream(st):
+                out = torch.empty(rows, dtype=torch.int32, device=dev)
+        _need(out, "out", torch.int32, dev)
+        if out.numel() != rows:
+            raise ValueError("out must have one entry per row")
+        rc = lib.tvp_sample_tokens(_ptr(logits), rows, vocab, max(logits.stride(0), vocab),
+                                   _ptr(uniforms), _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                                   _ptr(min_p), _ptr(out), _stream(st))
+    N.check(rc, "tvp_sample_tokens")
+    return out
+
+
 _EPILOGUES = {"bf16": 0, "f32": 1, "residual": 2, "swiglu": 3}
 
 
