@@ -498,7 +498,7 @@ int tvp_paged_window_prefill_attention(const tvp_bf16* q, const tvp_bf16* k_pool
  * rounded to BF16.  d_logits: [rows][row_stride], row_stride >= vocab; vocab at
  * most TVP_SAMPLE_MAX_VOCAB.  No workspace.
  */
-#define TVP_SAMPLE_MAX_VOCAB 393216
+#define TVP_SAMPLE_MAX_VOCAB 327680
 int tvp_sample_tokens(const float* d_logits, int rows, int vocab, long long row_stride,
                       const float* d_uniforms, const float* d_temperature, const int32_t* d_top_k,
                       const float* d_top_p, const float* d_min_p, int32_t* d_tokens,

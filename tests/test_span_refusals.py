@@ -63,7 +63,7 @@ def test_sampler_refuses(native):
         ({"logits": None}, INVALID), ({"u": None}, INVALID), ({"tokens": None}, INVALID), ({"rows": 0}, INVALID),
         ({"vocab": 0}, INVALID), ({"row_stride": 99}, INVALID), ({"logits": ctypes.c_void_p(0x10002)}, INVALID),
         ({"rows": 65536}, UNSUPPORTED),
-        ({"vocab": 393217, "row_stride": 393217}, UNSUPPORTED)])
+        ({"vocab": 327681, "row_stride": 327681}, UNSUPPORTED)])
 
 
 def test_span_workspace_bytes(native):
