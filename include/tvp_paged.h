@@ -409,11 +409,11 @@ int tvp_head_gather_destroy(tvp_head_gather* g);
 /*
  * Workspace of the two decode entry points below, for up to `batch` rows and
  * `groups` prefix groups (0: window decode only) on `num_ctas` CTAs (0 = one
- * per SM).  256-byte aligned, a multiple of 4 bytes in size, zeroed once
- * before its first use: every launch leaves its arrival counters zero.  One
- * workspace serves calls of any batch, groups and kv_heads that fit it; calls
- * that share it must not overlap on the GPU, and after a TVP_DEVERR_TIMEOUT it
- * must be zeroed again.  0 for arguments out of range.
+ * per SM, 1024 at most).  256-byte aligned, zeroed once before its first use:
+ * every launch leaves its arrival counters zero.  One workspace serves calls of
+ * any batch, groups, kv_heads and num_ctas that fit it; calls that share it
+ * must not overlap on the GPU, and after a TVP_DEVERR_TIMEOUT it must be zeroed
+ * again.  0 for arguments out of range.
  */
 size_t tvp_span_workspace_bytes(int batch, int groups, int kv_heads, int num_ctas);
 

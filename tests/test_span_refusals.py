@@ -28,8 +28,7 @@ COMMON = [({"q": None}, INVALID), ({"k": None}, INVALID), ({"v": None}, INVALID)
           ({"kvh": 3, "qh": 12}, UNSUPPORTED), ({"kvh": 16, "qh": 64}, UNSUPPORTED), ({"qh": 16}, UNSUPPORTED),
           ({"pages": 1 << 24}, UNSUPPORTED), ({"k": ODD}, INVALID), ({"out": ODD}, INVALID)]
 ROWS = [({"lens": None}, INVALID), ({"batch": 0}, INVALID), ({"batch": -1}, INVALID), ({"ctas": -1}, INVALID),
-        ({"ctas": 1025}, INVALID), ({"ws": None}, WORKSPACE), ({"wsb": 1 << 10}, WORKSPACE), ({"ws": ODD}, WORKSPACE),
-        ({"wsb": (1 << 30) + 1}, WORKSPACE)]
+        ({"ctas": 1025}, INVALID), ({"ws": None}, WORKSPACE), ({"wsb": 1 << 10}, WORKSPACE), ({"ws": ODD}, WORKSPACE)]
 WIN = [({"window": 0}, INVALID), ({"window": -5}, INVALID), ({"sinks": -1}, INVALID)]
 
 

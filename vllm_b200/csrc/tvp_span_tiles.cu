@@ -1,0 +1,594 @@
+// The tcgen05 tile kernel of K8 (prefill with a sliding window and sinks) and
+// of K7's shared prefixes: 32 query tokens of one KV head against a list of
+// pages, 128 MMA rows 4 t + h, so every K/V byte serves 4 heads of 32 tokens.
+//
+//   * PREFIX: the 32 tokens are 32 rows of a group, the pages a part of its
+//     prefix ("piece"); the CTA leaves (m, l, O) per (row, head) for the decode
+//     kernel to fold in.  The pieces' length is the shortest that keeps their
+//     number within piece_target (two CTAs per SM), so a few long prefixes and
+//     many short ones both fill the GPU once; every CTA works this out from the
+//     group sizes, a search of some ten steps by one warp.
+//   * window: the tokens are a tile of a sequence's queries, the pages the ones
+//     that some query of the tile sees; the CTA writes the output rows.
+//
+// Keys go in chunks of 4 pages (64 keys): warp 0 streams K and V boxes (TMA)
+// into a ring, one thread of warp 1 issues S = Q K^T and O += P V, two softmax
+// sides of four warps (one thread per row) take the chunks in turn, each with
+// its own S, P and O in Tensor Memory and its own running maximum and sum;
+// they merge at the end.  Unlike K3's, scores stay FP32, and P goes back into
+// the Tensor Memory columns of the scores it came from (two BF16 per column)
+// and is the MMA's A operand there: shared memory carries no P, whose write and
+// reads took half of its bandwidth (per 64-key chunk and tile 16 KB written and
+// 16 KB read, next to 24 KB for S, 8 KB for V and 16 KB from TMA).
+// The MMA thread issues S(0), S(1), then per chunk c: [wait P(c)] P V(c),
+// S(c + 2).  S(c)'s commit covers every earlier MMA, so when side c % 2 sees
+// S(c), P V(c - 2) has read P(c - 2), which S(c) overwrote, and written O.
+#include "tvp_span.cuh"
+#include "tvp_tile.cuh"
+#include "tvp_umma.cuh"
+
+namespace tvp {
+namespace {
+
+constexpr int kRows = kTileRows * kGroup;          // 128 MMA rows
+constexpr int kChunk = kChunkPages * kPage;        // 64 keys
+constexpr int kStages = 5;
+constexpr int kKvBytes = kChunkPages * kTileBytes;  // 8 KiB of K (or of V) per stage
+constexpr int kChunkBytes = 2 * kKvBytes;
+constexpr int kQBytes = kRows * 128;
+constexpr int kThreads = 12 * 32;
+// S / P of side 0: 0-63, of side 1: 64-127; O of side 0: 128-191, of side 1: 192-255
+constexpr uint32_t kTmemCols = 256;
+constexpr int kLowRegs = 32;    // warps 0-3
+constexpr int kHighRegs = 104;  // the softmax warps
+constexpr int kMinChunks = 2;   // a piece of a prefix is no shorter than this
+
+constexpr int kOffStages = kQBytes;
+constexpr int kOffBars = kOffStages + kStages * kChunkBytes;
+// q_full, o_full, drain, (unused), s_full[2], p_full[2], kv_full[stages], kv_empty[stages]
+constexpr int kBarSFull = 4;
+constexpr int kBarPFull = 6;
+constexpr int kBarKvFull = 8;
+constexpr int kBarKvEmpty = kBarKvFull + kStages;
+constexpr int kNumBars = kBarKvEmpty + kStages;
+constexpr int kOffPlan = kOffBars + kNumBars * 8 + 16;
+constexpr size_t kSmem = kOffPlan + 32;
+
+struct Piece {
+  int group, tile, head, first, last;  // pages [first, last) of the prefix
+};
+
+// Streams (tiles x KV heads) and chunks of group g; no streams without either.
+__device__ __forceinline__ int2 group_work(const SpanParams& p, int g) {
+  const int rows = __ldg(p.group_rows + g + 1) - __ldg(p.group_rows + g);
+  const int pages = shared_pages(p, g, false);
+  const int chunks = (pages + kChunkPages - 1) / kChunkPages;
+  return make_int2(chunks > 0 ? (rows + kTileRows - 1) / kTileRows * p.kv_heads : 0, chunks);
+}
+
+// Piece `index` of the prefixes, by one warp; group < 0 past the last.  The
+// first block also leaves every group's first piece and count of pieces per
+// stream for the decode kernel.
+__device__ __forceinline__ Piece find_piece(const SpanParams& p, int index, int lane, bool publish) {
+  auto sum = [](long long v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  long long streams = 0, work = 0;
+  int most = 1;
+  for (int g = lane; g < p.groups; g += 32) {
+    const int2 w = group_work(p, g);
+    streams += w.x;
+    work += (long long)w.x * w.y;
+    if (w.x > 0) most = max(most, w.y);
+  }
+  streams = sum(streams);
+  work = sum(work);
+  most = __reduce_max_sync(0xffffffffu, most);
+  const long long limit = streams > p.piece_target ? streams : p.piece_target;
+  // the shortest length whose pieces fit the limit, between the even share and
+  // one piece per stream
+  long long at_least = (work + limit - 1) / limit;
+  int lo = (int)(at_least > kMinChunks ? at_least : kMinChunks), hi = max(most, lo);
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    long long n = 0;
+    for (int g = lane; g < p.groups; g += 32) {
+      const int2 w = group_work(p, g);
+      n += (long long)w.x * ((w.y + mid - 1) / mid);
+    }
+    if (sum(n) <= limit)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  Piece out = {-1, 0, 0, 0, 0};
+  int before = 0;
+  for (int base = 0; base < p.groups; base += 32) {
+    const int g = base + lane;
+    const int2 w = g < p.groups ? group_work(p, g) : make_int2(0, 0);
+    const int splits = (w.y + lo - 1) / lo;
+    const int n = w.x * splits;
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    const int first = before + inc - n;
+    if (publish && g < p.groups) p.group_pieces[g] = make_int2(first, n > 0 ? splits : 0);
+    const bool here = index >= first && index < first + n;
+    const uint32_t who = __ballot_sync(0xffffffffu, here);
+    if (who) {
+      const int src = __ffs(who) - 1;
+      const int at = index - __shfl_sync(0xffffffffu, first, src);
+      const int k = __shfl_sync(0xffffffffu, splits, src);
+      const int chunks = __shfl_sync(0xffffffffu, w.y, src);
+      const int stream = at / k, j = at % k;
+      out.group = base + src;
+      out.tile = stream / p.kv_heads;
+      out.head = stream % p.kv_heads;
+      const int pages = shared_pages(p, out.group, false);
+      out.first = (int)((long long)chunks * j / k) * kChunkPages;
+      out.last = min(pages, (int)((long long)chunks * (j + 1) / k) * kChunkPages);
+      if (!publish) return out;
+    }
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return out;
+}
+
+template <bool PREFIX>
+__global__ void __launch_bounds__(kThreads, 2)
+    span_tiles_kernel(const SpanParams p, const __grid_constant__ CUtensorMap k_map,
+                      const __grid_constant__ CUtensorMap v_map) {
+  // 128-byte swizzled tiles need 1 KiB alignment (checked, as in K3).
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const uint32_t sbase = smem_addr(smem);
+  if (sbase & 1023u) {
+    if (threadIdx.x == 0) record_error(p.err, TVP_DEVERR_SMEM_ALIGN);
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int s, g, tok0, count, pos0 = 0, pos_last = 0;
+  int v_begin, v_end;  // pages of the list that this CTA takes
+  RowSpan span = {};   // window: from list to logical pages
+  const int32_t* table;
+  if (PREFIX) {
+    // The decode kernel may take the SMs that run out of pieces.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (!groups_in_order(p)) return;  // the decode kernel reports it
+    Piece* shared_piece = reinterpret_cast<Piece*>(smem + kOffPlan);
+    if (warp == 0) {
+      const bool publish = blockIdx.x == 0;
+      const Piece mine = find_piece(p, blockIdx.x, lane, publish);
+      if (lane == 0) *shared_piece = mine;
+      if (publish)
+        for (int i = lane; i < p.groups; i += 32) shared_pages(p, i, true);
+    }
+    __syncthreads();
+    const Piece piece = *shared_piece;
+    if (piece.group < 0) return;
+    s = piece.group;
+    g = piece.head;
+    const int r0 = __ldg(p.group_rows + s);
+    tok0 = r0 + piece.tile * kTileRows;
+    count = min(kTileRows, __ldg(p.group_rows + s + 1) - tok0);
+    v_begin = piece.first;
+    v_end = piece.last;
+    table = p.prefix_tables + (size_t)s * p.prefix_stride;
+  } else {
+    s = blockIdx.x;
+    g = blockIdx.y;
+    const int q_begin = __ldg(p.cu_q + s), q_end = __ldg(p.cu_q + s + 1);
+    const int tile = gridDim.z - 1 - blockIdx.z;  // the later tiles see the most keys
+    tok0 = q_begin + tile * kTileRows;
+    if (tok0 >= q_end) return;  // this sequence has fewer tiles
+    count = min(kTileRows, q_end - tok0);
+    pos0 = __ldg(p.q_pos0 + s) + tile * kTileRows;  // position of the tile's token 0
+    pos_last = pos0 + count - 1;
+    if (pos0 < 0 || pos_last / kPage >= p.table_stride) {
+      if (threadIdx.x == 0) record_error(p.err, TVP_DEVERR_BAD_TOKEN);
+      return;
+    }
+    span = window_span(pos_last + 1, (long long)pos0 + 1 - p.window, p.sinks);
+    v_begin = 0;
+    v_end = span.pages;
+    table = p.tables + (size_t)s * p.table_stride;
+  }
+  const int n_chunks = (v_end - v_begin + kChunkPages - 1) / kChunkPages;
+
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
+  auto bar = [&](int i) { return smem_addr(&bars[i]); };
+  const uint32_t q_full = bar(0), o_full = bar(1), drain = bar(2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int quarters = (count * kGroup + 31) / 32;  // row quarters with a real row
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 4);
+    mbar_init(o_full, 1);
+    mbar_init(drain, 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar(kBarSFull + b), 1);
+      mbar_init(bar(kBarPFull + b), quarters);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(bar(kBarKvFull + i), 1);
+      mbar_init(bar(kBarKvEmpty + i), 1);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_addr(tmem_slot), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  // Threads that meet before Tensor Memory is released: warp 1 and both sides.
+  constexpr int kEndThreads = 32 + 8 * 32;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLowRegs));
+    if (warp >= 2) return;  // the rest of this warpgroup only hands its registers over
+  }
+
+  if (warp == 0) {
+    // ------------------------------ producer ------------------------------
+    if (lane == 0) {
+      prefetch_tensor_map(&k_map);
+      prefetch_tensor_map(&v_map);
+    }
+    // lanes 0-3: K box of page slot `lane`, lanes 4-7: V box of slot lane - 4;
+    // the next chunk's page ids are loaded one chunk ahead.
+    auto page_id = [&](int c) {
+      const int v = v_begin + c * kChunkPages + (lane & 3);
+      return lane < 8 && v < v_end ? __ldg(table + span.logical(v)) : -1;
+    };
+    int issued = 0;
+    int next = page_id(0);
+    for (int c = 0; c < n_chunks; ++c) {
+      const int st = c % kStages;
+      const int phys = next;
+      if (c + 1 < n_chunks) next = page_id(c + 1);
+      if (c >= kStages) {
+        int timed_out = 0;
+        if (lane == 0) timed_out = !mbar_wait_bounded(bar(kBarKvEmpty + st), ((c / kStages) - 1) & 1);
+        if (__shfl_sync(0xffffffffu, timed_out, 0)) {
+          if (lane == 0) {
+            *abort_flag = 1;
+            record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_EMPTY);
+          }
+          break;
+        }
+      }
+      const bool real = lane < 8 && v_begin + c * kChunkPages + (lane & 3) < v_end;
+      const bool ok = real && phys >= 0 && phys < p.num_pages;
+      if (real && !ok && lane < 4) record_error(p.err, TVP_DEVERR_BAD_PAGE);
+      if (lane == 0) mbar_arrive_expect_tx(bar(kBarKvFull + st), kChunkBytes);
+      __syncwarp();
+      if (lane < 8) {
+        const uint32_t dst = sbase + kOffStages + st * kChunkBytes + (lane < 4 ? 0 : kKvBytes) +
+                             (lane & 3) * kTileBytes;
+        // A box wholly outside the pool (rows -16 .. -1) arrives as zeros.
+        const int y = ok ? (int)(p.layer_row_base + (long long)phys * kPage) : -kPage;
+        tma_load_2d(dst, lane < 4 ? &k_map : &v_map, g * kHeadDim, y, bar(kBarKvFull + st));
+      }
+      issued = c + 1;
+    }
+    drain_issued_stages<kStages>(bars + kBarKvFull, issued, lane, p.err);
+    return;
+  }
+
+  if (warp == 1) {
+    // ------------------------------ MMA issuer ----------------------------
+    if (lane == 0) {
+      constexpr uint32_t kIdS = umma_idesc_bf16_f32(kRows, kChunk, false, false);
+      constexpr uint32_t kIdO = umma_idesc_bf16_f32(kRows, kHeadDim, false, true);
+      auto stage_k = [&](int c) { return sbase + kOffStages + (c % kStages) * kChunkBytes; };
+      bool ok = true;
+      auto wait = [&](uint32_t b, uint32_t parity) {
+        if (ok && !mbar_wait_bounded(b, parity)) {
+          record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_FULL);
+          ok = false;
+        }
+        return ok;
+      };
+      // S(c) = Q K(c)^T into the columns of side c % 2, 16 channels per MMA.
+      auto issue_s = [&](int c) {
+        if (!wait(bar(kBarKvFull + c % kStages), (c / kStages) & 1)) return;
+        tc_fence_after_sync();
+        const uint32_t k_tile = stage_k(c);
+#pragma unroll
+        for (int k = 0; k < kHeadDim / 16; ++k)
+          umma_bf16(tmem + 64 * (c & 1), umma_desc_sw128(sbase + 32 * k, 16, 1024),
+                    umma_desc_sw128(k_tile + 32 * k, 16, 1024), kIdS, k > 0);
+        umma_commit(bar(kBarSFull + (c & 1)));
+      };
+      wait(q_full, 0);
+      issue_s(0);
+      if (n_chunks > 1) issue_s(1);
+      for (int c = 0; ok && c < n_chunks; ++c) {
+        // O_{c % 2} += P(c) V(c), 16 keys (one page of V, 8 columns of P) per
+        // MMA; the first chunk of each side overwrites its accumulator.
+        if (!wait(bar(kBarPFull + (c & 1)), (c >> 1) & 1)) break;
+        tc_fence_after_sync();
+        const uint32_t v_tile = stage_k(c) + kKvBytes;
+#pragma unroll
+        for (int kk = 0; kk < kChunkPages; ++kk)
+          umma_bf16_ts(tmem + 128 + 64 * (c & 1), tmem + 64 * (c & 1) + 8 * kk,
+                       umma_desc_sw128(v_tile + kk * kTileBytes, 0, 1024), kIdO, (c >= 2 || kk > 0));
+        umma_commit(bar(kBarKvEmpty + c % kStages));
+        if (c + 2 < n_chunks) issue_s(c + 2);
+      }
+      if (ok) umma_commit(o_full);
+      if (!ok) *abort_flag = 1;
+      // Every MMA issued has completed before Tensor Memory is released.
+      umma_commit(drain);
+      if (!mbar_wait_bounded(drain, 0))
+        record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_DRAIN);
+    }
+    __syncwarp();
+    tc_fence_before_sync();
+    named_barrier_sync(1, kEndThreads);
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
+
+  // ------------------------------ softmax sides ----------------------------
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHighRegs));
+  const int side = (warp - 4) >> 2;  // 0: warps 4-7 (even chunks), 1: warps 8-11 (odd)
+  const int quarter = warp & 3;      // TMEM lanes 32 quarter .. + 31
+  const int row = quarter * 32 + lane;
+  const int t = row >> 2, h = row & 3;
+  const bool valid = t < count;
+  const int qpos = pos0 + t;
+  const int qdim = p.kv_heads * kGroup * kHeadDim;
+  const int hq = g * kGroup + h;
+  const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+  // The exponent's factor must be positive for the maximum of the scores to be
+  // that of the products: a negative scale goes into q's sign, a zero one into q.
+  const float c_log2 = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  if (side == 0) {
+    // Q row (token t, head hq) into the swizzled A tile of S = Q K^T.
+    const uint4* src =
+        reinterpret_cast<const uint4*>(p.q + (size_t)(tok0 + t) * qdim + hq * kHeadDim);
+    const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+    const bool take = valid && p.scale_log2 != 0.f;
+#pragma unroll
+    for (int cc = 0; cc < 8; ++cc) {
+      uint4 w = take ? __ldg(src + cc) : make_uint4(0, 0, 0, 0);
+      w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
+      *reinterpret_cast<uint4*>(smem + sw128_offset(row, cc)) = w;
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_full);
+  }
+  const bool active = quarter < quarters;
+  float m = -INFINITY, l = 0.f;  // this side's running max (base-2 units) and normaliser
+  bool ok = true;
+  for (int c = side; active && c < n_chunks; c += 2) {
+    bool ready = !*abort_flag && mbar_wait_bounded(bar(kBarSFull + side), (c >> 1) & 1);
+    ready = __all_sync(0xffffffffu, ready);
+    if (!ready) {
+      if (lane == 0 && !*abort_flag) {
+        *abort_flag = 1;
+        record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_FULL);
+      }
+      ok = false;
+      break;
+    }
+    tc_fence_after_sync();
+    uint32_t sr[2][32];
+    tmem_ld32(tmem + 64 * side + lane_base, sr[0]);
+    tmem_ld32(tmem + 64 * side + 32 + lane_base, sr[1]);
+    tmem_wait_ld();
+    // Hidden keys: only chunks that are not seen whole by every row need the test.
+    const int v0 = v_begin + c * kChunkPages;
+    bool whole = v0 + kChunkPages <= v_end;
+    if (!PREFIX) {
+#pragma unroll
+      for (int i = 0; i < kChunkPages; ++i) {
+        const int t0 = span.logical(v0 + i) * kPage;
+        whole = whole && t0 + kPage - 1 <= pos0 &&
+                ((long long)t0 > (long long)pos_last - p.window || t0 + kPage <= p.sinks);
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < kChunkPages; ++i) {
+        uint32_t keep = 0u;
+        if (v0 + i < v_end) {
+          keep = 0xffffu;
+          if (!PREFIX) {
+            const RowSpan mine = {0, 0, 0, qpos + 1, p.sinks, max(0, qpos + 1 - p.window)};
+            keep = mine.keep(span.logical(v0 + i));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kPage; ++j)
+          if (!((keep >> j) & 1u)) sr[i >> 1][(i & 1) * kPage + j] = 0xff800000u;  // -inf
+      }
+    }
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        mx[e] = max3(mx[e], __uint_as_float(sr[0][j + e]), __uint_as_float(sr[1][j + e]));
+    }
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c_log2;
+    // Lazy running max: rescale only when a score beats the side's max by more
+    // than kLazyMargin (probabilities stay below 2^kLazyMargin).
+    float alpha = 1.f;
+    if (top > m + kLazyMargin) {
+      alpha = m == -INFINITY ? 0.f : fast_exp2(m - top);
+      m = top;
+    }
+    if (c >= 2 && __any_sync(0xffffffffu, alpha != 1.f)) {
+      // O_side holds this side's earlier chunks: S(c)'s commit, just waited
+      // for, covered P V(c - 2), the last MMA into it.
+#pragma unroll 1
+      for (int part = 0; part < 4; ++part) {
+        const uint32_t taddr = tmem + 128 + 64 * side + 16 * part + lane_base;
+        uint32_t o[16];
+        tmem_ld16(taddr, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+        tmem_st16(taddr, o);
+      }
+    }
+    const float nbase = m == -INFINITY ? 0.f : -m;
+    const uint64_t l2e2 = f2_pack(c_log2, c_log2), nb2 = f2_pack(nbase, nbase);
+    uint64_t ls2[4];  // four independent paired sums
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ls2[i] = f2_pack(0.f, 0.f);
+    // P over the scores' own columns, two keys per column.
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t w[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint64_t arg = f2_fma(f2_pack(__uint_as_float(sr[half][2 * j]),
+                                            __uint_as_float(sr[half][2 * j + 1])),
+                                    l2e2, nb2);
+        float a0, a1;
+        f2_unpack(arg, a0, a1);
+        const float p0 = fast_exp2(a0), p1 = fast_exp2(a1);
+        ls2[j & 3] = f2_add(ls2[j & 3], f2_pack(p0, p1));
+        w[j] = pack_bf16x2(p0, p1);
+      }
+      tmem_st16(tmem + 64 * side + 16 * half + lane_base, w);
+    }
+    tmem_wait_st();
+    float la, lb;
+    f2_unpack(f2_add(f2_add(ls2[0], ls2[1]), f2_add(ls2[2], ls2[3])), la, lb);
+    l = l * alpha + (la + lb);
+    // Tokens that no row of the tile sees may hold anything: zero them in the V
+    // tile before P V reads it (P is 0 there, but 0 x NaN is not).
+    if (!PREFIX && !whole && quarter == 0) {
+      const RowSpan any = {0, 0, 0, pos_last + 1, p.sinks, max(0, pos0 + 1 - p.window)};
+#pragma unroll
+      for (int i = 0; i < kChunkPages; ++i) {
+        if (v0 + i >= v_end) break;
+        const uint32_t keep = any.keep(span.logical(v0 + i));
+        if (keep != 0xffffu)
+          zero_hidden_v_rows(smem + kOffStages + (c % kStages) * kChunkBytes + kKvBytes +
+                                 i * kTileBytes, keep, lane);
+      }
+      fence_proxy_async_smem();
+    }
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(kBarPFull + side));
+  }
+  bool fin = active && ok && !*abort_flag && mbar_wait_bounded(o_full, 0);
+  fin = __all_sync(0xffffffffu, fin);
+  if (active && !fin && ok && lane == 0 && !*abort_flag) {
+    *abort_flag = 1;
+    record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_FULL);
+  }
+  // Merge the two sides per row: side 1 hands its (max, normaliser) to side 0
+  // through the Q tile, whose last reader (an S MMA) completed before o_full.
+  float* xchg = reinterpret_cast<float*>(smem);
+  if (side == 1 && fin) {
+    xchg[2 * row] = m;
+    xchg[2 * row + 1] = l;
+  }
+  named_barrier_sync(2, 8 * 32);
+  if (side == 0 && fin) {
+    const float mb = xchg[2 * row], lb = xchg[2 * row + 1];
+    const float mt = fmaxf(m, mb);
+    const float wa = m == -INFINITY ? 0.f : fast_exp2(m - mt);
+    const float wb = mb == -INFINITY ? 0.f : fast_exp2(mb - mt);
+    const float lt = l * wa + lb * wb;
+    const float inv = PREFIX ? 1.f : lt > 0.f ? 1.f / lt : 0.f;
+    const bool two = n_chunks > 1;  // side 1 wrote its accumulator
+    float* part = PREFIX ? p.pieces + ((size_t)blockIdx.x * kTileRows + t) * kPartialFloats : nullptr;
+    if (PREFIX && valid) {
+      part[h] = mt;
+      part[kGroup + h] = lt;
+    }
+    tc_fence_after_sync();
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t oa[32], ob[32];
+      tmem_ld32(tmem + 128 + 32 * half + lane_base, oa);
+      if (two) tmem_ld32(tmem + 192 + 32 * half + lane_base, ob);
+      tmem_wait_ld();
+      if (!valid) continue;
+      float x[32];
+#pragma unroll
+      for (int d = 0; d < 32; ++d) {
+        x[d] = __uint_as_float(oa[d]) * wa;
+        if (two) x[d] = fmaf(__uint_as_float(ob[d]), wb, x[d]);
+      }
+      if (PREFIX) {
+        float4* dst = reinterpret_cast<float4*>(part + 2 * kGroup + h * kHeadDim + 32 * half);
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+          dst[d] = make_float4(x[4 * d], x[4 * d + 1], x[4 * d + 2], x[4 * d + 3]);
+      } else {
+        uint4* dst = reinterpret_cast<uint4*>(p.out + (size_t)(tok0 + t) * qdim + hq * kHeadDim) +
+                     4 * half;
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc)
+          dst[cc] = make_uint4(pack_bf16x2(x[8 * cc] * inv, x[8 * cc + 1] * inv),
+                               pack_bf16x2(x[8 * cc + 2] * inv, x[8 * cc + 3] * inv),
+                               pack_bf16x2(x[8 * cc + 4] * inv, x[8 * cc + 5] * inv),
+                               pack_bf16x2(x[8 * cc + 6] * inv, x[8 * cc + 7] * inv));
+      }
+    }
+  }
+  tc_fence_before_sync();
+  named_barrier_sync(1, kEndThreads);
+}
+
+template <bool PREFIX>
+cudaError_t launch_tiles(const SpanParams& p, long long pool_rows, dim3 grid, cudaStream_t stream) {
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    // A register split that the launch's pool cannot satisfy would never return.
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, span_tiles_kernel<PREFIX>);
+    if (e != cudaSuccess) return e;
+    if ((long long)fa.numRegs * kThreads < 128LL * kLowRegs + 256LL * kHighRegs)
+      return cudaErrorInvalidConfiguration;
+    e = cudaFuncSetAttribute(span_tiles_kernel<PREFIX>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  CUtensorMap k_map, v_map;
+  if (!pool_tensor_map(p.k_pool, pool_rows, p.kv_heads, &k_map) ||
+      !pool_tensor_map(p.v_pool, pool_rows, p.kv_heads, &v_map))
+    return cudaErrorInvalidValue;
+  span_tiles_kernel<PREFIX><<<grid, kThreads, kSmem, stream>>>(p, k_map, v_map);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_prefix_tiles(const SpanParams& p, long long pool_rows, int max_pieces,
+                                cudaStream_t stream) {
+  return launch_tiles<true>(p, pool_rows, dim3((unsigned)max_pieces), stream);
+}
+
+cudaError_t launch_window_tiles(const SpanParams& p, long long pool_rows, int max_q_len,
+                                int num_seqs, cudaStream_t stream) {
+  return launch_tiles<false>(
+      p, pool_rows,
+      dim3((unsigned)num_seqs, (unsigned)p.kv_heads, (unsigned)((max_q_len + kTileRows - 1) / kTileRows)),
+      stream);
+}
+
+}  // namespace tvp

@@ -118,6 +118,16 @@ __device__ __forceinline__ void zero_stale_v_rows(unsigned char* vtile, int vali
   }
 }
 
+// The rows of a V tile whose bit in `keep` is 0, as zero_stale_v_rows.
+__device__ __forceinline__ void zero_hidden_v_rows(unsigned char* vtile, uint32_t keep, int lane) {
+#pragma unroll
+  for (int e = 0; e < kPage * 8 / 32; ++e) {
+    const int idx = lane + 32 * e, r = idx >> 3;
+    if (!((keep >> r) & 1u))
+      *reinterpret_cast<uint4*>(vtile + r * 128 + (idx & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // K and V fragments of one tile (shared addresses of its K and V tiles).
 __device__ __forceinline__ void load_tile_frags(uint32_t ktile, uint32_t vtile, const TileLane& tl,
                                                 uint32_t kf[4][4], uint32_t vf[4][4]) {
@@ -132,12 +142,13 @@ __device__ __forceinline__ void load_tile_frags(uint32_t ktile, uint32_t vtile, 
 }
 
 // One tile into the online softmax: scores, (lazy) running max, BF16
-// probabilities, P.V accumulation.  `valid` = tokens of the tile inside the
-// sequence (rows >= valid are masked).
+// probabilities, P.V accumulation.  With `partial`, the tile's tokens tr and
+// tr + 8 count only where keep_a and keep_b say so.
 template <bool LAZY>
-__device__ __forceinline__ void attend_tile(HeadState& st, const uint32_t kf[4][4],
-                                            const uint32_t vf[4][4], const uint32_t qb[4][2],
-                                            int valid, const TileLane& tl, float scale_log2) {
+__device__ __forceinline__ void attend_tile_keep(HeadState& st, const uint32_t kf[4][4],
+                                                 const uint32_t vf[4][4], const uint32_t qb[4][2],
+                                                 bool partial, bool keep_a, bool keep_b,
+                                                 float scale_log2) {
   // S^T = K Q^T, as two independent accumulation chains (channels 0-31, 32-63)
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
   float t0 = 0.f, t1 = 0.f, t2 = 0.f, t3 = 0.f;
@@ -150,9 +161,9 @@ __device__ __forceinline__ void attend_tile(HeadState& st, const uint32_t kf[4][
   }
   float x0 = (s0 + t0) * scale_log2, x1 = (s1 + t1) * scale_log2;
   float x2 = (s2 + t2) * scale_log2, x3 = (s3 + t3) * scale_log2;
-  if (valid < kPage) {
-    if (tl.tr >= valid) x0 = x1 = -INFINITY;
-    if (tl.tr + 8 >= valid) x2 = x3 = -INFINITY;
+  if (partial) {
+    if (!keep_a) x0 = x1 = -INFINITY;
+    if (!keep_b) x2 = x3 = -INFINITY;
   }
   float mx0 = fmaxf(x0, x2), mx1 = fmaxf(x1, x3);
   // LAZY keeps the running maximum unless a score beats it by more than
@@ -189,6 +200,15 @@ __device__ __forceinline__ void attend_tile(HeadState& st, const uint32_t kf[4][
   for (int d = 0; d < 4; ++d)
     mma_bf16_16816(st.acc[d][0], st.acc[d][1], st.acc[d][2], st.acc[d][3], vf[d][0], vf[d][1],
                    vf[d][2], vf[d][3], y0, y1);
+}
+
+// `valid` = tokens of the tile inside the sequence (rows >= valid are masked).
+template <bool LAZY>
+__device__ __forceinline__ void attend_tile(HeadState& st, const uint32_t kf[4][4],
+                                            const uint32_t vf[4][4], const uint32_t qb[4][2],
+                                            int valid, const TileLane& tl, float scale_log2) {
+  attend_tile_keep<LAZY>(st, kf, vf, qb, valid < kPage, tl.tr < valid, tl.tr + 8 < valid,
+                         scale_log2);
 }
 
 // Sums the per-lane partial normalisers over the token rows.
@@ -385,27 +405,33 @@ __device__ __forceinline__ void combine_partials(const float* partials, int grou
   out.store16(h * kHeadDim + d0, packed);
 }
 
-// Publishes a partial piece; true in every lane when it is the last piece of
-// its sequence to arrive (a counter per (sequence, KV head group), reset by
-// the last arriver for the next launch; no waiting).
-__device__ __forceinline__ bool publish_partial(const HeadState& st, float* partials, int* counters,
-                                                int groups, int g, int s, int slot, int first,
-                                                int end, long long T, long long R,
-                                                const TileLane& tl, int lane) {
-  write_partial(st, partials + ((size_t)slot * groups + g) * kPartialFloats, tl);
+// Publishes a partial piece at `part`; true in every lane when it is the last
+// of its sequence's `pieces` to arrive (one counter per (sequence, KV head
+// group), reset by the last arriver for the next launch; no waiting).
+__device__ __forceinline__ bool publish_partial_at(const HeadState& st, float* part, int* counter,
+                                                   int pieces, const TileLane& tl, int lane) {
+  write_partial(st, part, tl);
   __threadfence();
   __syncwarp();
   int last = 0;
   if (lane == 0) {
-    const int pieces = range_of_page(end - 1, T, R) - range_of_page(first, T, R) + 1;
-    const int old = atomicAdd(counters + (size_t)s * groups + g, 1);
+    const int old = atomicAdd(counter, 1);
     last = (old == pieces - 1);
     if (last) {
-      atomicExch(counters + (size_t)s * groups + g, 0);
+      atomicExch(counter, 0);
       __threadfence();
     }
   }
   return __shfl_sync(0xffffffffu, last, 0) != 0;
+}
+
+__device__ __forceinline__ bool publish_partial(const HeadState& st, float* partials, int* counters,
+                                                int groups, int g, int s, int slot, int first,
+                                                int end, long long T, long long R,
+                                                const TileLane& tl, int lane) {
+  return publish_partial_at(st, partials + ((size_t)slot * groups + g) * kPartialFloats,
+                            counters + (size_t)s * groups + g,
+                            range_of_page(end - 1, T, R) - range_of_page(first, T, R) + 1, tl, lane);
 }
 
 // Publishes a partial piece and, when it is the last of its sequence to arrive,
