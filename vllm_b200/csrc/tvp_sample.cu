@@ -7,21 +7,23 @@
 // Weights.  w_i = exp((x_i - max) / T) is held as an integer of 2^-44 of the
 // largest weight, so sums are exact in any order (atomics included) and every
 // CTA count gives the same token; a vocabulary of 2^19 ones sums below 2^63.
-// FP32 exponentials would not do: with 2^17 logits the running sum's borders
-// lie closer together than 2^-24 of the whole.  2^-t is taken in FP64: t in
-// 32nds of an octave, a table of the 32 fractions and a Taylor polynomial of
-// degree 5 (|f| <= 1/64 octave: the first term left out is below 2^-48).
+// Plain FP32 exponentials would not do: with 2^17 logits the running sum's
+// borders lie closer together than 2^-24 of the whole.  2^-t is taken with t in
+// 256ths of an octave, a table of the 256 fractions and a Taylor polynomial of
+// degree 3 (|f| <= 1/512 octave: the first term left out is below 2^-42).
 //
 // Filters.  top-k and top-p cut the row at a place in its falling order (value,
 // then index).  A histogram of the distance from the maximum, 2048 buckets over
 // the distances that still have weight, finds the bucket of the cut; each CTA
 // bins its eighth, CTA r adds up buckets [256 r, 256 r + 256) of all eight
 // through distributed shared memory.  When few enough logits lie at or above
-// that bucket (a usual nucleus), CTA 0 gathers and sorts them, cuts and draws:
-// 4 cluster barriers in all.  Otherwise only the cut's own bucket is gathered
-// and sorted (or, when equal logits fill it, resolved by radix digits and an
-// index count), and the draw goes by sums: per CTA, per warp, then within the
-// warp's segment in index order.
+// that bucket (a usual nucleus), CTA 0 gathers them, cuts and draws, all by
+// comparing each with each; 4 cluster barriers in all.  Otherwise only the cut's
+// own bucket is gathered (or, when it holds many, resolved by radix digits and a
+// count of equal logits by index), and the draw goes by sums: per CTA, per warp,
+// then within the warp's segment in index order.
+#include <cfloat>
+
 #include <cooperative_groups.h>
 
 #include "tvp_common.cuh"
@@ -37,7 +39,9 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBuckets = 2048;
 constexpr int kSegment = kBuckets / kCluster;
-constexpr int kList = 2048;  // logits that CTA 0 sorts
+constexpr int kBlocks = kBuckets / 32;  // two per lane of a warp
+static_assert(kBlocks == 64 && kSegment <= kThreads, "border() deals them out so");
+constexpr int kList = 512;  // logits that CTA 0 takes in
 constexpr int kFixedBits = 44;
 // Distances (in units of T) past which a weight rounds to 0: 45 ln 2.
 constexpr float kFar = 31.25f;
@@ -51,20 +55,39 @@ struct alignas(16) Shared {
   u64 best[kCluster];  // by rank: (order image, ~index) of the largest logit
   float least[kCluster];
   u64 amount[kCluster];  // by rank: a sum that the step at hand exchanges
-  u64 count[kCluster];
-  u64 fills[kCluster];
+  int fills[kCluster];
   u64 ties[kCluster];
-  u64 seg[kSegment];       // this CTA's segment of the cluster's histogram: amounts
+  u64 seg[kSegment];         // this CTA's segment of the cluster's histogram: amounts
   uint32_t seg_n[kSegment];  // and counts
+  u64 sub[kBlocks];          // every 32 buckets of the cluster's histogram: amounts
+  uint32_t sub_n[kBlocks];   // and counts
   u64 warp[kWarps];
-  u64 found[4];
-  double pow[32];  // 2^(-j / 32)
+  float warp_lo[kWarps];
+  u64 found;
+  double pow[256];
   Cut cut;
   int fill;
 };
 
-constexpr size_t kScratchBytes = 2 * kList * 8;  // histogram, then the lists
-static_assert(kScratchBytes >= kBuckets * 12, "the histogram fits the lists' place");
+// 2^(-j / 256), by the Taylor series of the exponential.
+struct Powers {
+  double d[256];
+  constexpr Powers() : d() {
+    for (int j = 0; j < 256; ++j) {
+      const double x = -j * (0.6931471805599453 / 256);
+      double term = 1, sum = 1;
+      for (int n = 1; n < 24; ++n) {
+        term *= x / n;
+        sum += term;
+      }
+      d[j] = sum;
+    }
+  }
+};
+__device__ const Powers g_powers = Powers();
+
+constexpr size_t kScratchBytes = kBuckets * 12;  // histogram, then the lists
+static_assert(kScratchBytes >= 3 * kList * 8, "the lists fit the histogram's place");
 
 __device__ __forceinline__ uint32_t order_of(float x) {  // larger logit, larger image
   const uint32_t u = __float_as_uint(x);
@@ -79,13 +102,24 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ u64 warp_scan(u64 v, int lane) {  // inclusive
+template <typename V>
+__device__ __forceinline__ V warp_scan(V v, int lane) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const u64 y = __shfl_up_sync(0xffffffffu, v, o);
+    const V y = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += y;
   }
   return v;
+}
+
+// 64-bit sum into shared memory from two 32-bit ones: the low words' carry goes
+// with the high word, which most weights do not touch.
+__device__ __forceinline__ void shared_add(u64* at, u64 w) {
+  uint32_t* p = reinterpret_cast<uint32_t*>(at);
+  const uint32_t lo = (uint32_t)w;
+  uint32_t hi = (uint32_t)(w >> 32);
+  if (lo) hi += atomicAdd(p, lo) > ~lo;
+  if (hi) atomicAdd(p + 1, hi);
 }
 
 struct Sampler {
@@ -95,35 +129,51 @@ struct Sampler {
   unsigned char* scratch;
   int rank, begin, len;
   int tid, lane, warp;
-  float top;
-  double c32;   // 32 log2(e) / T
+  float top;    // finite
+  float far;    // logits below it have no weight
+  double c256;  // 256 log2(e) / T
   float scale;  // buckets per unit of distance
+  bool cutting;  // a filter has cut the row
+  Cut cut;
 
-  __device__ u64 fixed(float v) const {  // weight of a logit above -inf, in 2^-44
-    if (v == top) return 1ull << kFixedBits;
-    const double t = ((double)top - (double)v) * c32;
-    if (!(t <= 32.0 * (kFixedBits + 1))) return 0;
+  // Weight of a logit in 2^-44 of the largest's.  Without branches, so that the
+  // chains of several logits overlap.  (An FP32 form that carries the products'
+  // rounding errors along, good to 2^-31, measured the same time: 11 FP64
+  // instructions against some 30 FP32 ones.)
+  __device__ __forceinline__ u64 fixed(float v) const {
+    const double t = ((double)top - (double)fmaxf(v, far)) * c256;
     const double shifted = t + 6755399441055744.0;  // 1.5 * 2^52: rounds to an integer
     const int k = __double2loint(shifted);
-    const double f = ((shifted - 6755399441055744.0) - t) * (0.6931471805599453 / 32.0);
-    double y = fma(f, 1.0 / 120.0, 1.0 / 24.0);
-    y = fma(y, f, 1.0 / 6.0);
-    y = fma(y, f, 0.5);
+    const double f = ((shifted - 6755399441055744.0) - t) * (0.6931471805599453 / 256);
+    double y = fma(f, 1.0 / 6.0, 0.5);
     y = fma(y, f, 1.0);
     y = fma(y, f, 1.0);
-    y *= s.pow[k & 31];
-    // * 2^(44 - k / 32), then the integer part from the sum's mantissa
-    y = fma(y, __hiloint2double((1023 + kFixedBits - (k >> 5)) << 20, 0), 4503599627370496.0);
-    return (u64)__double_as_longlong(y) & 0xfffffffffffffull;
+    y *= s.pow[k & 255];
+    // * 2^(44 - k / 256), then the integer part from the sum's mantissa
+    y = fma(y, __hiloint2double((1023 + kFixedBits - (k >> 8)) << 20, 0), 4503599627370496.0);
+    return v < far ? 0ull : (u64)__double_as_longlong(y) & 0xfffffffffffffull;
   }
-  __device__ int bucket(float v) const {  // rises as v falls
-    if (v == top) return 0;  // also +inf, whose distance is no number
+  __device__ __forceinline__ int bucket(float v) const {  // rises as v falls
     return (int)fminf((top - v) * scale, (float)(kBuckets - 1));
   }
-  __device__ bool kept(float v, int i) const {
-    if (!(v > -INFINITY)) return false;
+  __device__ __forceinline__ bool kept(float v, int i) const {
+    if (!cutting) return v > -INFINITY;
     const uint32_t o = order_of(v);
-    return o > s.cut.key || (o == s.cut.key && i <= s.cut.last);
+    return o > cut.key || (o == cut.key && i <= cut.last);
+  }
+  // Calls visit(logit, index in the CTA's part) for the CTA's logits, four
+  // neighbours of a thread at a time.
+  template <typename Visit>
+  __device__ __forceinline__ void each_logit(Visit visit) const {
+    const int n4 = len / 4;
+    for (int q = tid; q < n4; q += kThreads) {
+      const float4 v = reinterpret_cast<const float4*>(x)[q];
+      visit(v.x, 4 * q);
+      visit(v.y, 4 * q + 1);
+      visit(v.z, 4 * q + 2);
+      visit(v.w, 4 * q + 3);
+    }
+    if (tid < len - 4 * n4) visit(x[4 * n4 + tid], 4 * n4 + tid);
   }
 
   // Exclusive sum over the block's threads (all must call), and the total.
@@ -142,139 +192,163 @@ struct Sampler {
   // Every CTA's value, to every CTA's `place[rank]`; a cluster barrier inside.
   // Between two calls with one place every CTA passes another cluster barrier
   // after its reads.
-  __device__ void share(u64* place, u64 v) {
+  template <typename V>
+  __device__ void share(V* place, V v) {
     if (tid < kCluster) cluster.map_shared_rank(place, tid)[rank] = v;
     cluster.sync();
   }
 
   // Histogram of the logits that `take` accepts, by `bin` (0 first in falling
-  // order): the bin where the running amount reaches want(total); returns the
-  // bin, the amount before it, and the counts before and in it.
+  // order): the bin where the running amount reaches want(total), the amount
+  // before it, and the counts before and in it (0: the amount is not reached).
   struct Border {
     int bin;
-    u64 above, want, above_n, in_n;
+    u64 above, want;
+    int above_n, in_n;
   };
-  template <typename Take, typename Bin, typename Want>
-  __device__ Border border(bool mass, Take take, Bin bin, Want want_of) {
+  template <bool MASS, typename Take, typename Bin, typename Want>
+  __device__ Border border(Take take, Bin bin, Want want_of) {
     u64* hist = reinterpret_cast<u64*>(scratch);
     uint32_t* hist_n = reinterpret_cast<uint32_t*>(hist + kBuckets);
     for (int i = tid; i < kBuckets; i += kThreads) {
-      hist[i] = 0;
+      if (MASS) hist[i] = 0;
       hist_n[i] = 0;
     }
     __syncthreads();
-    for (int i = tid; i < len; i += kThreads) {
-      const float v = x[i];
-      if (!take(v, begin + i)) continue;
+    auto add = [&](float v, u64 w, int i) {
+      if (!take(v, begin + i)) return;
       const int b = bin(v);
       atomicAdd(&hist_n[b], 1u);
-      if (mass) {
-        const u64 w = fixed(v);
-        if (w) atomicAdd(&hist[b], w);
+      if (MASS) shared_add(&hist[b], w);
+    };
+    const int n4 = len / 4;
+    for (int q = tid; q < n4; q += kThreads) {
+      const float4 v = reinterpret_cast<const float4*>(x)[q];
+      u64 w[4] = {};
+      if (MASS) {
+        w[0] = fixed(v.x);
+        w[1] = fixed(v.y);
+        w[2] = fixed(v.z);
+        w[3] = fixed(v.w);
+      }
+      add(v.x, w[0], 4 * q);
+      add(v.y, w[1], 4 * q + 1);
+      add(v.z, w[2], 4 * q + 2);
+      add(v.w, w[3], 4 * q + 3);
+    }
+    if (tid < len - 4 * n4) {
+      const float v = x[4 * n4 + tid];
+      add(v, MASS ? fixed(v) : 0, 4 * n4 + tid);
+    }
+    cluster.sync();
+    // This CTA's segment over all eight, one bucket per thread of 8 warps, and
+    // the sum of each warp's 32 to every CTA.
+    if (tid < kSegment) {
+      const int b = rank * kSegment + tid;
+      uint32_t ns[kCluster];
+      u64 as[kCluster];
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r) {
+        ns[r] = cluster.map_shared_rank(hist_n, r)[b];
+        if (MASS) as[r] = cluster.map_shared_rank(hist, r)[b];
+      }
+      uint32_t n = 0;
+      u64 a = 0;
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r) {
+        n += ns[r];
+        a += MASS ? as[r] : ns[r];
+      }
+      s.seg[tid] = a;
+      s.seg_n[tid] = n;
+      a = MASS ? warp_sum(a) : 0;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane < kCluster) {
+        cluster.map_shared_rank(s.sub, lane)[rank * (kSegment / 32) + warp] = MASS ? a : n;
+        cluster.map_shared_rank(s.sub_n, lane)[rank * (kSegment / 32) + warp] = n;
       }
     }
     cluster.sync();
-    // This CTA's segment over all eight.
-    u64 a = 0, n = 0;
-    if (tid < kSegment) {
-      const int b = rank * kSegment + tid;
-#pragma unroll
-      for (int r = 0; r < kCluster; ++r) {
-        n += cluster.map_shared_rank(hist_n, r)[b];
-        if (mass) a += cluster.map_shared_rank(hist, r)[b];
-      }
-      if (!mass) a = n;
-      s.seg[tid] = a;
-      s.seg_n[tid] = (uint32_t)n;
-    }
-    u64 all, all_n;
-    block_scan(a, &all);
-    block_scan(n, &all_n);
-    if (tid < kCluster) cluster.map_shared_rank(s.count, tid)[rank] = all_n;
-    share(s.amount, all);
-    u64 total = 0;
-#pragma unroll
-    for (int r = 0; r < kCluster; ++r) total += s.amount[r];
+    // Every warp finds the 32 buckets, then the bucket, for itself.
     Border out;
-    out.want = want_of(total);
-    out.above = out.above_n = 0;
-    int seg = 0;
-    for (; seg < kCluster - 1 && out.above + s.amount[seg] < out.want; ++seg) {
-      out.above += s.amount[seg];
-      out.above_n += s.count[seg];
+    const u64 s0 = s.sub[2 * lane], s1 = s.sub[2 * lane + 1];
+    const uint32_t n0 = s.sub_n[2 * lane], n1 = s.sub_n[2 * lane + 1];
+    const u64 inc = warp_scan(s0 + s1, lane);
+    const uint32_t inc_n = warp_scan(n0 + n1, lane);
+    out.want = want_of(__shfl_sync(0xffffffffu, inc, 31));
+    const u64 before = inc - s0 - s1;
+    const uint32_t at = __ballot_sync(0xffffffffu, before < out.want && inc >= out.want);
+    if (at == 0) {
+      out.bin = kBuckets - 1;
+      out.above = __shfl_sync(0xffffffffu, inc, 31);
+      out.above_n = (int)__shfl_sync(0xffffffffu, inc_n, 31);
+      out.in_n = 0;
+      return out;
     }
-    const u64 ba = tid < kSegment ? cluster.map_shared_rank(s.seg, seg)[tid] : 0;
-    const u64 bn = tid < kSegment ? cluster.map_shared_rank(s.seg_n, seg)[tid] : 0;
-    const u64 before = block_scan(ba, &all) + out.above;
-    const u64 before_n = block_scan(bn, &all_n) + out.above_n;
-    if (tid == 0) {  // amounts that never reach `want`: the last bin of all
-      s.found[0] = kBuckets - 1;
-      s.found[1] = out.above + all;
-      s.found[2] = out.above_n + all_n;
-      s.found[3] = 0;
-    }
-    __syncthreads();
-    if (tid < kSegment && before < out.want && before + ba >= out.want) {
-      s.found[0] = seg * kSegment + tid;
-      s.found[1] = before;
-      s.found[2] = before_n;
-      s.found[3] = bn;
-    }
-    __syncthreads();
-    out.bin = (int)s.found[0];
-    out.above = s.found[1];
-    out.above_n = s.found[2];
-    out.in_n = s.found[3];
+    const int src = __ffs(at) - 1;
+    const bool second = before + s0 < out.want;
+    const int block = 2 * src + __shfl_sync(0xffffffffu, (int)second, src);
+    const u64 above = __shfl_sync(0xffffffffu, second ? before + s0 : before, src);
+    const uint32_t above_n =
+        __shfl_sync(0xffffffffu, second ? inc_n - n1 : inc_n - n0 - n1, src);
+    constexpr int kPer = kSegment / 32;  // blocks of a CTA
+    const int place = block % kPer * 32 + lane;
+    const u64 ba = cluster.map_shared_rank(s.seg, block / kPer)[place];
+    const uint32_t bn = cluster.map_shared_rank(s.seg_n, block / kPer)[place];
+    const u64 upto = above + warp_scan(ba, lane);
+    const uint32_t upto_n = above_n + warp_scan(bn, lane);
+    const int hit = __ffs(__ballot_sync(0xffffffffu, upto >= out.want)) - 1;
+    out.bin = block * 32 + hit;
+    out.above = __shfl_sync(0xffffffffu, upto - ba, hit);
+    out.above_n = (int)__shfl_sync(0xffffffffu, upto_n - bn, hit);
+    out.in_n = (int)__shfl_sync(0xffffffffu, bn, hit);
     return out;
   }
 
-  // The logits that `take` accepts, as (order image, ~index), in CTA 0's list
-  // sorted falling; n of them in the cluster (n <= kList).  Only CTA 0 returns
-  // true.
+  // The n (<= kList) logits that `take` accepts, as (order image, ~index), in
+  // CTA 0's list, in no order.  Only CTA 0 returns true.
+  __device__ u64* list() const { return reinterpret_cast<u64*>(scratch) + kList; }
+  __device__ u64* weights() const { return reinterpret_cast<u64*>(scratch) + 2 * kList; }
   template <typename Take>
-  __device__ bool gather_sorted(Take take, int n) {
+  __device__ bool gather(Take take, int n) {
     u64* mine = reinterpret_cast<u64*>(scratch);
     if (tid == 0) s.fill = 0;
     __syncthreads();
-    for (int i = tid; i < len; i += kThreads) {
-      const float v = x[i];
-      if (!take(v, begin + i)) continue;
-      mine[atomicAdd(&s.fill, 1)] = ((u64)order_of(v) << 32) | (uint32_t)~(begin + i);
+    each_logit([&](float v, int i) {
+      if (take(v, begin + i))
+        mine[atomicAdd(&s.fill, 1)] = ((u64)order_of(v) << 32) | (uint32_t)~(begin + i);
+    });
+    __syncthreads();
+    share(s.fills, s.fill);
+    if (rank != 0) return false;
+    if (tid < n) {
+      int r = 0, at = tid;
+#pragma unroll
+      for (int q = 0; q < kCluster - 1; ++q)
+        if (r == q && at >= s.fills[q]) {
+          at -= s.fills[q];
+          ++r;
+        }
+      list()[tid] = cluster.map_shared_rank(mine, r)[at];
     }
     __syncthreads();
-    share(s.fills, (u64)s.fill);
-    if (rank != 0) return false;
-    u64* list = mine + kList;
-    int at = 0;
-    for (int r = 0; r < kCluster; ++r) {
-      const u64* from = cluster.map_shared_rank(mine, r);
-      const int m = (int)s.fills[r];
-      for (int i = tid; i < m; i += kThreads) list[at + i] = from[i];
-      at += m;
-    }
-    sort_falling(list, n);
     return true;
   }
 
-  // Bitonic sort of list[0..n), padded with zeros to a power of two.
-  __device__ void sort_falling(u64* list, int n) {
-    int size = 2;
-    while (size < n) size <<= 1;
-    for (int i = n + tid; i < size; i += kThreads) list[i] = 0;
-    __syncthreads();
-    for (int k = 2; k <= size; k <<= 1) {
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        for (int p = tid; p < size / 2; p += kThreads) {
-          const int i = 2 * p - (p & (j - 1));
-          const u64 a = list[i], b = list[i + j];
-          if ((a < b) == ((i & k) == 0)) {
-            list[i] = b;
-            list[i + j] = a;
-          }
-        }
-        __syncthreads();
-      }
-    }
+  // The list is not sorted: an entry's place in the falling order is what lies
+  // ahead of it, counted by `parts` threads per entry.
+  struct Share {
+    int parts, i, q;  // threads per entry, this thread's entry, its part
+  };
+  __device__ Share share_of(int n) const {
+    int parts = 32;
+    while (kThreads / parts < n) parts >>= 1;
+    return {parts, tid / parts, tid % parts};
+  }
+  template <typename V>
+  __device__ static V over_parts(V v, int parts) {
+    for (int o = 1; o < parts; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
   }
 
   // The integer that a running sum must exceed: u of `total` (> 0).
@@ -289,95 +363,73 @@ struct Sampler {
     return w < 1.0 ? 1ull : (u64)w;
   }
 
-  // CTA 0: the token among its sorted list[0..n) (the largest logits, falling):
-  // at most the first m, of these the shortest run that weighs `want` (0: the
-  // share P of their whole), min-p M, draw u.
-  __device__ void finish(const u64* list, int m, u64 want, float P, float M, float u,
-                         int32_t* token) {
-    constexpr int kEach = kList / kThreads;
-    u64* by_index = reinterpret_cast<u64*>(scratch);  // the local list, read before the sort
-    // weights in falling order; thread t holds kEach neighbours
-    u64 w[kEach], mine = 0, total;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = tid * kEach + e;
-      w[e] = i < m ? fixed(of_order((uint32_t)(list[i] >> 32))) : 0;
-      mine += w[e];
-    }
-    u64 before = block_scan(mine, &total);
-    if (want == 0) want = P < 1.f ? want_of(P, total) : ~0ull;
-    int r = 0;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = tid * kEach + e;
-      if (i < m && (i == 0 || before < want) && !below(list[i], M)) r = i + 1;
-      before += w[e];
-    }
-    if (tid == 0) s.fill = 0;
+  // CTA 0: the token among its list of n (the largest logits): at most the
+  // first k (0: all), of these the shortest run that weighs `want` (0: the share
+  // P of their whole), min-p M, draw u.
+  __device__ void finish(int n, int k, u64 want, float P, float M, float u, int32_t* token) {
+    const u64* entries = list();
+    u64* w = weights();
+    if (tid < n) w[tid] = fixed(of_order((uint32_t)(entries[tid] >> 32)));
     __syncthreads();
-    r = __reduce_max_sync(0xffffffffu, r);
-    if (lane == 0) atomicMax(&s.fill, r);
-    __syncthreads();
-    r = s.fill;
-    // in index order: sort ~index (falling), which keeps the place in the list
-    for (int i = tid; i < r; i += kThreads)
-      by_index[i] = ((list[i] & 0xffffffffull) << 32) | (uint32_t)i;
-    __syncthreads();
-    sort_falling(by_index, r);
-    mine = 0;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = tid * kEach + e;
-      w[e] = i < r ? fixed(of_order((uint32_t)(list[(uint32_t)by_index[i]] >> 32))) : 0;
-      mine += w[e];
+    const Share sh = share_of(n);
+    const bool mine = sh.i < n;
+    const u64 me = mine ? entries[sh.i] : 0, weight = mine ? w[sh.i] : 0;
+    int ahead = 0;
+    u64 mass = 0, total;
+    for (int j = sh.q; j < n; j += sh.parts)
+      if (entries[j] > me) {
+        ++ahead;
+        mass += w[j];
+      }
+    ahead = over_parts(ahead, sh.parts);
+    mass = over_parts(mass, sh.parts);
+    bool keep = mine && (k == 0 || ahead < k);
+    if (want == 0) {
+      block_scan(keep && sh.q == 0 ? weight : 0, &total);
+      want = P < 1.f ? want_of(P, total) : ~0ull;
     }
-    before = block_scan(mine, &total);
+    keep = keep && (ahead == 0 || mass < want) && !below(of_order((uint32_t)(me >> 32)), M);
+    block_scan(keep && sh.q == 0 ? weight : 0, &total);  // and every thread has read w
+    if (mine && sh.q == 0 && !keep) w[sh.i] = 0;
+    __syncthreads();
+    // the running sum in index order
+    u64 lower = 0;
+    for (int j = sh.q; j < n; j += sh.parts) lower += (uint32_t)entries[j] > (uint32_t)me ? w[j] : 0;
+    lower = over_parts(lower, sh.parts);
     const u64 point = point_of(u, total);
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = tid * kEach + e;
-      if (w[e] && before <= point && before + w[e] > point)
-        *token = (int32_t)~(uint32_t)(by_index[i] >> 32);
-      before += w[e];
-    }
+    if (keep && sh.q == 0 && lower <= point && lower + weight > point)
+      *token = (int32_t)~(uint32_t)me;
   }
-  __device__ bool below(u64 entry, float M) const {
-    return M > 0.f && below(of_order((uint32_t)(entry >> 32)), M);
-  }
-  __device__ bool below(float v, float M) const {  // exp((v - top) / T) < M
-    return v != top && exp(((double)v - (double)top) * (c32 * (0.6931471805599453 / 32.0))) < (double)M;
+  __device__ __forceinline__ bool below(float v, float M) const {  // exp((v - top) / T) < M
+    return M > 0.f && v != top &&
+           exp(((double)v - (double)top) * (c256 * (0.6931471805599453 / 256))) < (double)M;
   }
 
-  // The cut in bucket `b` (gathered, sorted when it fits) or, for a bucket of
-  // more logits, by radix digits of the order image and, among equal logits,
-  // by index.  `need`: the amount still wanted of that bucket.
-  __device__ void cut_in_bucket(bool mass, int bkt, u64 need, u64 in_n) {
-    auto inside = [&](float v, int i) { return kept(v, i) && bucket(v) == bkt; };
+  // The cut in bucket `bkt`: among its logits gathered, or, for a bucket of
+  // many, by radix digits of the order image and, among equal logits, by index.
+  // `need`: the amount still wanted of that bucket.
+  template <bool MASS>
+  __device__ void cut_in_bucket(int bkt, u64 need, int in_n) {
+    auto inside = [&](float v, int i) { return bucket(v) == bkt && kept(v, i); };
     if (in_n <= kList) {
-      if (gather_sorted(inside, (int)in_n)) {
-        constexpr int kEach = kList / kThreads;
-        const u64* list = reinterpret_cast<u64*>(scratch) + kList;
-        u64 w[kEach], mine = 0, total;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          const int i = tid * kEach + e;
-          w[e] = i < (int)in_n ? (mass ? fixed(of_order((uint32_t)(list[i] >> 32))) : 1) : 0;
-          mine += w[e];
-        }
-        u64 before = block_scan(mine, &total);
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          const int i = tid * kEach + e;
-          if (w[e] && before < need && before + w[e] >= need) s.found[0] = list[i];
-          before += w[e];
-        }
+      if (gather(inside, in_n)) {
+        const u64* entries = list();
+        u64* w = weights();
+        if (tid < in_n) w[tid] = MASS ? fixed(of_order((uint32_t)(entries[tid] >> 32))) : 1;
         __syncthreads();
-        if (tid < kCluster) {
-          const Cut c = {(uint32_t)(s.found[0] >> 32), (int)~(uint32_t)s.found[0]};
-          *cluster.map_shared_rank(&s.cut, tid) = c;
+        const Share sh = share_of(in_n);
+        const u64 me = sh.i < in_n ? entries[sh.i] : 0;
+        u64 ahead = 0;
+        for (int j = sh.q; j < in_n; j += sh.parts) ahead += entries[j] > me ? w[j] : 0;
+        ahead = over_parts(ahead, sh.parts);
+        if (sh.i < in_n && sh.q == 0 && ahead < need && ahead + w[sh.i] >= need) {
+          const Cut c = {(uint32_t)(me >> 32), (int)~(uint32_t)me};
+          for (int r = 0; r < kCluster; ++r) *cluster.map_shared_rank(&s.cut, r) = c;
         }
       }
       cluster.sync();
+      cut = s.cut;
+      cutting = true;
       return;
     }
     uint32_t prefix = 0, mask = 0;
@@ -385,8 +437,8 @@ struct Sampler {
     const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
     for (int d = 0; d < 3; ++d) {
       const uint32_t top_digit = (1u << bits[d]) - 1u;
-      const Border at = border(
-          mass, [&](float v, int i) { return inside(v, i) && (order_of(v) & mask) == prefix; },
+      const Border at = border<MASS>(
+          [&](float v, int i) { return inside(v, i) && (order_of(v) & mask) == prefix; },
           [&](float v) { return (int)(top_digit - ((order_of(v) >> shifts[d]) & top_digit)); },
           [&](u64) { return left; });
       prefix |= (top_digit - (uint32_t)at.bin) << shifts[d];
@@ -394,7 +446,7 @@ struct Sampler {
       left = at.want - at.above;
     }
     // `left` of the amount of equal logits: the n-th of them by index.
-    const u64 unit = mass ? fixed(of_order(prefix)) : 1;
+    const u64 unit = MASS ? fixed(of_order(prefix)) : 1;
     const u64 nth = (left + unit - 1) / unit;
     const int each = (len + kThreads - 1) / kThreads;
     const int i0 = min(tid * each, len), i1 = min(i0 + each, len);
@@ -408,10 +460,30 @@ struct Sampler {
     if (seen < nth && seen + ties >= nth)
       for (int i = i0; i < i1; ++i)
         if (kept(x[i], begin + i) && order_of(x[i]) == prefix && ++seen == nth) last = begin + i;
-    cluster.sync();  // every CTA has used the old cut
     if (last >= 0)
       for (int r = 0; r < kCluster; ++r) *cluster.map_shared_rank(&s.cut, r) = {prefix, last};
     cluster.sync();
+    cut = s.cut;
+    cutting = true;
+  }
+
+  // One filter: true when it ended the row (the token is written).
+  template <bool MASS, typename Want>
+  __device__ bool filter(Want want_of, int k, float P, float M, float u, int32_t* token) {
+    const Border at = border<MASS>([&](float v, int i) { return kept(v, i); },
+                                   [&](float v) { return bucket(v); }, want_of);
+    if (at.in_n == 0) return false;  // fewer logits above -inf than k
+    const int n = at.above_n + at.in_n;
+    if (n > kList) {
+      cut_in_bucket<MASS>(at.bin, at.want - at.above, at.in_n);
+      return false;
+    }
+    // After a histogram of weights the amount wanted is known, of the whole;
+    // after one of counts, top-p is of the k that are left.
+    if (gather([&](float v, int i) { return bucket(v) <= at.bin && kept(v, i); }, n))
+      finish(n, MASS ? 0 : k, MASS ? at.want : 0, P, M, u, token);
+    cluster.sync();  // CTA 0 reads the others' lists
+    return true;
   }
 };
 
@@ -427,14 +499,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int begin = min(rank * slice, vocab), len = min(slice, vocab - begin);
   float* x = reinterpret_cast<float*>(smem + kScratchBytes);
-  if (tid < 32) s.pow[tid] = exp2(-tid / 32.0);
-  if (tid == 0) s.cut = {0u, vocab};
-  const float T = temperature ? temperature[row] : 1.f;
-  const int k = top_k ? top_k[row] : 0;
-  const float P = top_p ? top_p[row] : 1.f;
-  const float mp = min_p ? min_p[row] : 0.f;
-  const float M = mp > 0.f ? fminf(mp, 1.f) : 0.f;
-  const float u = uniforms[row];
 
   // This CTA's logits into shared memory, and the row's largest and least.
   float hi = -INFINITY, lo = INFINITY;
@@ -493,16 +557,23 @@ __global__ void __launch_bounds__(kThreads, 2)
     best = c > best ? c : best;
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
   }
-  __shared__ float warp_lo[kWarps];
   if (lane == 0) {
     s.warp[warp] = best;
-    warp_lo[warp] = lo;
+    s.warp_lo[warp] = lo;
   }
+  if (tid < 256) s.pow[tid] = g_powers.d[tid];
+  float T = temperature ? temperature[row] : 1.f;
+  if (T > 0.f) T = fmaxf(T, 2e-36f);  // 256 log2(e) / T stays finite
+  const int k = top_k ? top_k[row] : 0;
+  const float P = top_p ? top_p[row] : 1.f;
+  const float mp = min_p ? min_p[row] : 0.f;
+  const float M = mp > 0.f ? fminf(mp, 1.f) : 0.f;
+  const float u = uniforms[row];
   __syncthreads();
   if (tid < kCluster) {
     for (int w = 0; w < kWarps; ++w) {
       best = s.warp[w] > best ? s.warp[w] : best;
-      lo = fminf(lo, warp_lo[w]);
+      lo = fminf(lo, s.warp_lo[w]);
     }
     cluster.map_shared_rank(s.best, tid)[rank] = best;
     cluster.map_shared_rank(s.least, tid)[rank] = lo;
@@ -519,47 +590,46 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (rank == 0 && tid == 0) tokens[row] = best == 0 ? -1 : (int32_t)~(uint32_t)best;
     return;
   }
-  const float top = of_order((uint32_t)(best >> 32));
+  float top = of_order((uint32_t)(best >> 32));
+  if (top == INFINITY) {  // these share the mass: zeros among -inf
+    for (int i = tid; i < len; i += kThreads) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
+    __syncthreads();
+    top = lo = 0.f;
+  }
   // Buckets over the distances that have weight, or over the row's own range
   // where that is narrower.
   const float range = fminf(kFar * T, top - lo);
+  const double c256 = 369.3299304675746 / (double)T;
   Sampler a = {cluster, s, x, smem, rank, begin, len, tid, lane, warp, top,
-               46.16624130844683 / (double)T, range > 0.f ? (float)kBuckets / range : 0.f};
-  const bool by_k = k > 0 && k < vocab;
-  if (by_k || P < 1.f) {
-    auto any = [&](float v, int i) { return a.kept(v, i); };
-    auto bin = [&](float v) { return a.bucket(v); };
-    for (int filter = by_k ? 0 : 1; filter < 2; ++filter) {
-      const bool mass = filter == 1;
-      if (mass && !(P < 1.f)) break;
-      const Sampler::Border at = a.border(mass, any, bin, [&](u64 total) {
-        return mass ? Sampler::want_of(P, total) : (u64)k;
-      });
-      const u64 n = at.above_n + at.in_n;
-      if (at.in_n == 0) continue;  // fewer logits above -inf than k
-      if (n <= kList) {
-        if (a.gather_sorted([&](float v, int i) { return a.kept(v, i) && a.bucket(v) <= at.bin; },
-                            (int)n)) {
-          // After a histogram of weights the amount wanted is known, of the
-          // whole; after one of counts, top-p is of the k that are left.
-          a.finish(reinterpret_cast<u64*>(smem) + kList, mass ? (int)n : min((int)n, k),
-                   mass ? at.want : 0, P, M, u, tokens + row);
-        }
-        cluster.sync();  // CTA 0 reads the others' lists
-        return;
-      }
-      a.cut_in_bucket(mass, at.bin, at.want - at.above, at.in_n);
-    }
-  }
+               fmaxf(top - kFar * T, -FLT_MAX), c256,
+               range > 0.f ? (float)kBuckets / range : 0.f, false, {}};
+  if (k > 0 && k < vocab &&
+      a.filter<false>([&](u64) { return (u64)k; }, k, P, M, u, tokens + row))
+    return;
+  if (P < 1.f && a.filter<true>([&](u64 total) { return Sampler::want_of(P, total); }, k, P, M, u,
+                                tokens + row))
+    return;
   // The draw by sums: warps take neighbouring segments of the CTA's logits.
+  // min-p: logits well above and below its distance need no exponential.
+  const float dist = M > 0.f ? (float)(-log((double)M) * (double)T) : 0.f;
   auto weight = [&](int i) -> u64 {
-    if (i >= len || !a.kept(x[i], begin + i) || (M > 0.f && a.below(x[i], M))) return 0;
-    return a.fixed(x[i]);
+    const float v = i < len ? x[i] : -INFINITY;
+    const u64 w = a.fixed(v);
+    if (M > 0.f) {
+      const float d = top - v;
+      if (d > dist * 1.00001f || (d >= dist * 0.99999f && a.below(v, M))) return 0;
+    }
+    return a.kept(v, begin + i) ? w : 0;
   };
-  const int part = (len + kWarps * 32 - 1) / (kWarps * 32) * 32;
+  const int part = (len + kWarps * 128 - 1) / (kWarps * 128) * 128;
   const int w0 = min(warp * part, len), w1 = min(w0 + part, len);
   u64 sum = 0;
-  for (int i = w0 + lane; i < w1; i += 32) sum += weight(i);
+  for (int i = w0 + 4 * lane; i < w1; i += 128) {
+    u64 w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = weight(i + e);  // 0 past the part's end
+    sum += (w[0] + w[1]) + (w[2] + w[3]);
+  }
   sum = warp_sum(sum);
   __syncthreads();
   if (lane == 0) s.warp[warp] = sum;
@@ -574,14 +644,21 @@ __global__ void __launch_bounds__(kThreads, 2)
     total += s.amount[r];
   }
   const u64 point = Sampler::point_of(u, total);
-  for (int w = 0; w < warp; ++w) before += s.warp[w];
-  if (before > point || before + sum <= point) return;
-  for (int i = w0; i < w1; i += 32) {
-    const u64 w = i + lane < w1 ? weight(i + lane) : 0;
-    const u64 inc = before + warp_scan(w, lane);
-    if (w && inc - w <= point && inc > point) tokens[row] = begin + i + lane;
-    before = __shfl_sync(0xffffffffu, inc, 31);
-    if (before > point) return;
+  if (before > point || before + mine <= point) return;
+  // The whole CTA goes over the segment that holds the point.
+  int seg = 0;
+  while (before + s.warp[seg] <= point) before += s.warp[seg++];
+  const int s0 = min(seg * part, len), s1 = min(s0 + part, len);
+  const int each = (s1 - s0 + kThreads - 1) / kThreads;
+  const int i0 = min(s0 + tid * each, s1), i1 = min(i0 + each, s1);
+  mine = 0;
+  for (int i = i0; i < i1; ++i) mine += weight(i);
+  u64 run = before + a.block_scan(mine, &total);
+  if (run > point || run + mine <= point) return;
+  for (int i = i0; i < i1; ++i) {
+    const u64 w = weight(i);
+    if (w && run <= point && run + w > point) tokens[row] = begin + i;
+    run += w;
   }
 }
 

@@ -260,44 +260,87 @@ class SpanWorkspace:
         self.buffer.zero_()
 
 
-def _on(dev, stream):
-    """The stream a call runs on: the given one, which must be of the tensors'
-    device, or that device's current one."""
-    if stream is None:
-        return torch.cuda.current_stream(dev)
-    if stream.device != dev:
-        raise ValueError(f"stream is of {stream.device}, the tensors are on {dev}")
-    return stream
+def _addr(t):
+    """A tensor's address for a call whose argument types are declared."""
+    return None if t is None else t.data_ptr()
 
 
-def _output(out, like, stream):
-    """``out``, or a tensor like ``like`` that belongs to the call's stream."""
-    if out is None:
-        with torch.cuda.stream(stream):
-            return torch.empty_like(like)
-    _need(out, "out", like.dtype, like.device)
-    if out.shape != like.shape:
-        raise ValueError(f"out must be {list(like.shape)}")
-    return out
+def _take(t, name, dtype, dev):
+    """`_need` with its checks in one test where they all hold."""
+    if t is None or t.dtype is not dtype or t.get_device() != dev.index or not t.is_contiguous():
+        _need(t, name, dtype, dev)
 
 
-def _need_error(error, dev):
-    if error is not None:
-        _need(error, "error", torch.int32, dev)
+class _Call:
+    """Where a call runs: the tensors' device made current (and the one before
+    restored), and the stream, the given one, which must be of that device, or
+    the device's current one."""
+
+    __slots__ = ("dev", "stream", "given", "before")
+
+    def __init__(self, dev, stream):
+        if stream is not None and stream.device != dev:
+            raise ValueError(f"stream is of {stream.device}, the tensors are on {dev}")
+        self.dev, self.given = dev, stream
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.dev.index:
+            torch.cuda.set_device(self.dev)
+        # the raw handle: making a Stream object of it takes 4 us
+        self.stream = (torch._C._cuda_getCurrentRawStream(self.dev.index) if self.given is None
+                       else self.given.cuda_stream)
+        return self
+
+    def __exit__(self, *exc):
+        if self.before != self.dev.index:
+            torch.cuda.set_device(self.before)
+
+    def empty_like(self, like, dtype):
+        """A tensor that belongs to the call's stream."""
+        if self.given is None:
+            return torch.empty_like(like, dtype=dtype)
+        with torch.cuda.stream(self.given):
+            return torch.empty_like(like, dtype=dtype)
+
+    def output(self, out, like, dtype):
+        """``out``, or a tensor shaped like ``like``."""
+        if out is None:
+            return self.empty_like(like, dtype)
+        _take(out, "out", dtype, self.dev)
+        if out.shape != like.shape:
+            raise ValueError(f"out must be {list(like.shape)}")
+        return out
 
 
-def _decode_rows(q, k_pool, v_pool, block_tables, seq_lens, workspace, error):
-    """Argument checks of the span decode calls; the pools' geometry."""
-    num_layers, num_pages, kv_heads = _pool_geometry(k_pool, v_pool)
+def _span_geometry(k_pool, v_pool, q, block_tables, error):
+    """Argument checks that the span calls share; the pools' geometry."""
     dev = k_pool.device
-    _need(q, "q", torch.bfloat16, dev)
-    _need(block_tables, "block_tables", torch.int32, dev)
-    _need(seq_lens, "seq_lens", torch.int32, dev)
-    _need_error(error, dev)
+    if k_pool.get_device() < 0:
+        _need(k_pool, "k_pool", torch.bfloat16)
+    _take(k_pool, "k_pool", torch.bfloat16, dev)
+    _take(v_pool, "v_pool", torch.bfloat16, dev)
+    shape = k_pool.shape
+    if len(shape) != 4 or shape != v_pool.shape or shape[2] != N.PAGE_TOKENS or shape[3] % N.HEAD_DIM:
+        raise ValueError("pools must be [num_layers, num_pages, 16, kv_heads*64] and equal")
+    _take(q, "q", torch.bfloat16, dev)
+    _take(block_tables, "block_tables", torch.int32, dev)
+    if error is not None:
+        _take(error, "error", torch.int32, dev)
+    if q.dim() != 2 or q.shape[1] != shape[3] * N.GQA_GROUP:
+        raise ValueError("q must be [tokens, 4*kv_heads*64]")
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be [rows, table_stride]")
+    return dev, shape[0], shape[1], shape[3] // N.HEAD_DIM
+
+
+def _decode_rows(kv_heads, dev, q, block_tables, seq_lens, workspace):
+    """Argument checks of the span decode calls; the number of rows."""
+    _take(seq_lens, "seq_lens", torch.int32, dev)
     batch = seq_lens.numel()
-    if q.shape != (batch, kv_heads * N.GQA_GROUP * N.HEAD_DIM):
-        raise ValueError("q must be [batch, 4*kv_heads*64]")
-    if block_tables.dim() != 2 or block_tables.shape[0] < batch:
+    if q.shape[0] != batch:
+        raise ValueError("q must have one row per entry of seq_lens")
+    if block_tables.shape[0] < batch:
         raise ValueError("block_tables must be [>=batch, table_stride]")
     if workspace is None or workspace.buffer.device != dev:
         raise ValueError("a SpanWorkspace on the tensors' device is required")
@@ -305,7 +348,7 @@ def _decode_rows(q, k_pool, v_pool, block_tables, seq_lens, workspace, error):
         raise ValueError(f"workspace was sized for {workspace.kv_heads} KV heads, pools hold {kv_heads}")
     if batch > workspace.max_batch:
         raise ValueError("batch larger than the workspace was sized for")
-    return num_layers, num_pages, kv_heads, batch
+    return batch
 
 
 def paged_window_decode_attention(q, k_pool, v_pool, layer, block_tables, seq_lens, window,
@@ -316,17 +359,15 @@ def paged_window_decode_attention(q, k_pool, v_pool, layer, block_tables, seq_le
     first ``sinks``; a row of length 0 gets zeros.  Pages without a visible token
     are not read (their table entries may be -1).  No plan is needed."""
     lib = N.load()
-    num_layers, num_pages, kv_heads, batch = _decode_rows(q, k_pool, v_pool, block_tables,
-                                                          seq_lens, workspace, error)
-    dev = k_pool.device
-    with torch.cuda.device(dev):
-        st = _on(dev, stream)
-        out = _output(out, q, st)
+    dev, num_layers, num_pages, kv_heads = _span_geometry(k_pool, v_pool, q, block_tables, error)
+    batch = _decode_rows(kv_heads, dev, q, block_tables, seq_lens, workspace)
+    with _Call(dev, stream) as call:
+        out = call.output(out, q, torch.bfloat16)
         rc = lib.tvp_paged_window_decode_attention(
-            _ptr(q), _ptr(k_pool), _ptr(v_pool), num_pages, num_layers, layer, kv_heads,
-            kv_heads * N.GQA_GROUP, _ptr(block_tables), block_tables.shape[1], _ptr(seq_lens),
+            _addr(q), _addr(k_pool), _addr(v_pool), num_pages, num_layers, layer, kv_heads,
+            kv_heads * N.GQA_GROUP, _addr(block_tables), block_tables.shape[1], _addr(seq_lens),
             batch, int(window), int(sinks), float(scale), workspace.num_ctas,
-            _ptr(workspace.buffer), workspace.nbytes, _ptr(out), _ptr(error), _stream(st))
+            _addr(workspace.buffer), workspace.nbytes, _addr(out), _addr(error), call.stream)
     N.check(rc, "tvp_paged_window_decode_attention")
     return out
 
@@ -341,12 +382,11 @@ def paged_shared_prefix_decode_attention(q, k_pool, v_pool, layer, block_tables,
     at their places (position / 16) in ``block_tables``.  prefix_tables: int32
     [groups, stride]; prefix_pages: int32 [groups]; group_rows: int32 [groups + 1]."""
     lib = N.load()
-    num_layers, num_pages, kv_heads, batch = _decode_rows(q, k_pool, v_pool, block_tables,
-                                                          seq_lens, workspace, error)
-    dev = k_pool.device
-    _need(prefix_tables, "prefix_tables", torch.int32, dev)
-    _need(prefix_pages, "prefix_pages", torch.int32, dev)
-    _need(group_rows, "group_rows", torch.int32, dev)
+    dev, num_layers, num_pages, kv_heads = _span_geometry(k_pool, v_pool, q, block_tables, error)
+    batch = _decode_rows(kv_heads, dev, q, block_tables, seq_lens, workspace)
+    _take(prefix_tables, "prefix_tables", torch.int32, dev)
+    _take(prefix_pages, "prefix_pages", torch.int32, dev)
+    _take(group_rows, "group_rows", torch.int32, dev)
     groups = prefix_pages.numel()
     if group_rows.numel() != groups + 1:
         raise ValueError("group_rows must have groups + 1 entries")
@@ -354,15 +394,14 @@ def paged_shared_prefix_decode_attention(q, k_pool, v_pool, layer, block_tables,
         raise ValueError("prefix_tables must be [>=groups, prefix_stride]")
     if groups > workspace.max_groups:
         raise ValueError("more groups than the workspace was sized for")
-    with torch.cuda.device(dev):
-        st = _on(dev, stream)
-        out = _output(out, q, st)
+    with _Call(dev, stream) as call:
+        out = call.output(out, q, torch.bfloat16)
         rc = lib.tvp_paged_shared_prefix_decode_attention(
-            _ptr(q), _ptr(k_pool), _ptr(v_pool), num_pages, num_layers, layer, kv_heads,
-            kv_heads * N.GQA_GROUP, _ptr(block_tables), block_tables.shape[1], _ptr(seq_lens),
-            batch, _ptr(prefix_tables), prefix_tables.shape[1], _ptr(prefix_pages),
-            _ptr(group_rows), groups, float(scale), workspace.num_ctas, _ptr(workspace.buffer),
-            workspace.nbytes, _ptr(out), _ptr(error), _stream(st))
+            _addr(q), _addr(k_pool), _addr(v_pool), num_pages, num_layers, layer, kv_heads,
+            kv_heads * N.GQA_GROUP, _addr(block_tables), block_tables.shape[1], _addr(seq_lens),
+            batch, _addr(prefix_tables), prefix_tables.shape[1], _addr(prefix_pages),
+            _addr(group_rows), groups, float(scale), workspace.num_ctas, _addr(workspace.buffer),
+            workspace.nbytes, _addr(out), _addr(error), call.stream)
     N.check(rc, "tvp_paged_shared_prefix_decode_attention")
     return out
 
@@ -373,30 +412,23 @@ def paged_window_prefill_attention(q, k_pool, v_pool, layer, block_tables, cu_q,
     sinks: the query at position p sees key j <= p when j > p - window or
     j < sinks."""
     lib = N.load()
-    num_layers, num_pages, kv_heads = _pool_geometry(k_pool, v_pool)
-    dev = k_pool.device
-    _need(q, "q", torch.bfloat16, dev)
-    _need(block_tables, "block_tables", torch.int32, dev)
-    _need(cu_q, "cu_q", torch.int32, dev)
-    _need(q_pos0, "q_pos0", torch.int32, dev)
-    _need_error(error, dev)
+    dev, num_layers, num_pages, kv_heads = _span_geometry(k_pool, v_pool, q, block_tables, error)
+    _take(cu_q, "cu_q", torch.int32, dev)
+    _take(q_pos0, "q_pos0", torch.int32, dev)
     num_seqs = q_pos0.numel()
     if cu_q.numel() != num_seqs + 1:
         raise ValueError("cu_q must have num_seqs + 1 entries")
-    if q.dim() != 2 or q.shape[1] != kv_heads * N.GQA_GROUP * N.HEAD_DIM:
-        raise ValueError("q must be [num_tokens, 4*kv_heads*64]")
-    if block_tables.dim() != 2 or block_tables.shape[0] < num_seqs:
+    if block_tables.shape[0] < num_seqs:
         raise ValueError("block_tables must be [>=num_seqs, table_stride]")
-    with torch.cuda.device(dev):
-        st = _on(dev, stream)
-        out = _output(out, q, st)
+    with _Call(dev, stream) as call:
+        out = call.output(out, q, torch.bfloat16)
         if q.shape[0] == 0:
             return out
         rc = lib.tvp_paged_window_prefill_attention(
-            _ptr(q), _ptr(k_pool), _ptr(v_pool), num_pages, num_layers, layer, kv_heads,
-            kv_heads * N.GQA_GROUP, _ptr(block_tables), block_tables.shape[1], _ptr(cu_q),
-            _ptr(q_pos0), num_seqs, int(max_q_len), int(window), int(sinks), float(scale),
-            _ptr(out), _ptr(error), _stream(st))
+            _addr(q), _addr(k_pool), _addr(v_pool), num_pages, num_layers, layer, kv_heads,
+            kv_heads * N.GQA_GROUP, _addr(block_tables), block_tables.shape[1], _addr(cu_q),
+            _addr(q_pos0), num_seqs, int(max_q_len), int(window), int(sinks), float(scale),
+            _addr(out), _addr(error), call.stream)
     N.check(rc, "tvp_paged_window_prefill_attention")
     return out
 
@@ -417,27 +449,21 @@ def sample_tokens(logits, uniforms, temperature=None, top_k=None, top_p=None, mi
         raise ValueError("logits must be [rows, vocab] with unit stride along vocab")
     rows, vocab = logits.shape
     dev = logits.device
-    _need(uniforms, "uniforms", torch.float32, dev)
+    _take(uniforms, "uniforms", torch.float32, dev)
     per_row = [(uniforms, "uniforms")]
     for t, name, dtype in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32),
                            (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
         if t is not None:
-            _need(t, name, dtype, dev)
+            _take(t, name, dtype, dev)
             per_row.append((t, name))
     for t, name in per_row:
         if t.numel() != rows:
             raise ValueError(f"{name} must have one entry per row")
-    with torch.cuda.device(dev):
-        st = _on(dev, stream)
-        if out is None:
-            with torch.cuda.stream(st):
-                out = torch.empty(rows, dtype=torch.int32, device=dev)
-        _need(out, "out", torch.int32, dev)
-        if out.numel() != rows:
-            raise ValueError("out must have one entry per row")
-        rc = lib.tvp_sample_tokens(_ptr(logits), rows, vocab, max(logits.stride(0), vocab),
-                                   _ptr(uniforms), _ptr(temperature), _ptr(top_k), _ptr(top_p),
-                                   _ptr(min_p), _ptr(out), _stream(st))
+    with _Call(dev, stream) as call:
+        out = call.output(out, uniforms, torch.int32)
+        rc = lib.tvp_sample_tokens(_addr(logits), rows, vocab, max(logits.stride(0), vocab),
+                                   _addr(uniforms), _addr(temperature), _addr(top_k), _addr(top_p),
+                                   _addr(min_p), _addr(out), call.stream)
     N.check(rc, "tvp_sample_tokens")
     return out
 
