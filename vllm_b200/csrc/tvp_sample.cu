@@ -41,7 +41,10 @@ constexpr int kBuckets = 2048;
 constexpr int kSegment = kBuckets / kCluster;
 constexpr int kBlocks = kBuckets / 32;  // two per lane of a warp
 static_assert(kBlocks == 64 && kSegment <= kThreads, "border() deals them out so");
-constexpr int kList = 512;  // logits that CTA 0 takes in
+constexpr int kList = 512;  // logits of a bucket that CTA 0 takes in
+// Logits at or above the cut that CTA 0 finishes by itself.  Each-with-each takes
+// 2 x 0.7 us for 128 and 2 x 11 us for 512; the sums take some 3 us of passes.
+constexpr int kFew = 160;
 constexpr int kFixedBits = 44;
 // Distances (in units of T) past which a weight rounds to 0: 45 ln 2.
 constexpr float kFar = 31.25f;
@@ -49,6 +52,13 @@ constexpr float kFar = 31.25f;
 struct Cut {
   uint32_t key;  // kept: order image above it, or equal and index <= last
   int last;
+};
+
+// The bin where a running amount reaches `want`: the amount before it, and the
+// counts before and in it (0: the amount is not reached).
+struct Border {
+  int bin, above_n, in_n;
+  u64 above, want;
 };
 
 struct alignas(16) Shared {
@@ -66,6 +76,7 @@ struct alignas(16) Shared {
   u64 found;
   double pow[256];
   Cut cut;
+  Border border;
   int fill;
 };
 
@@ -199,21 +210,13 @@ struct Sampler {
   }
 
   // Histogram of the logits that `take` accepts, by `bin` (0 first in falling
-  // order): the bin where the running amount reaches want(total), the amount
-  // before it, and the counts before and in it (0: the amount is not reached).
-  struct Border {
-    int bin;
-    u64 above, want;
-    int above_n, in_n;
-  };
+  // order), and the bin where the running amount reaches want(total).
   template <bool MASS, typename Take, typename Bin, typename Want>
   __device__ Border border(Take take, Bin bin, Want want_of) {
     u64* hist = reinterpret_cast<u64*>(scratch);
     uint32_t* hist_n = reinterpret_cast<uint32_t*>(hist + kBuckets);
-    for (int i = tid; i < kBuckets; i += kThreads) {
-      if (MASS) hist[i] = 0;
-      hist_n[i] = 0;
-    }
+    for (int i = tid; i < (int)(kScratchBytes / 16); i += kThreads)
+      reinterpret_cast<uint4*>(scratch)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     auto add = [&](float v, u64 w, int i) {
       if (!take(v, begin + i)) return;
@@ -225,7 +228,7 @@ struct Sampler {
     for (int q = tid; q < n4; q += kThreads) {
       const float4 v = reinterpret_cast<const float4*>(x)[q];
       u64 w[4] = {};
-      if (MASS) {
+      if (MASS && fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= far) {
         w[0] = fixed(v.x);
         w[1] = fixed(v.y);
         w[2] = fixed(v.z);
@@ -269,7 +272,13 @@ struct Sampler {
       }
     }
     cluster.sync();
-    // Every warp finds the 32 buckets, then the bucket, for itself.
+    // One warp finds the 32 buckets, then the bucket.
+    if (warp == 0) find_border(want_of);
+    __syncthreads();
+    return s.border;
+  }
+  template <typename Want>
+  __device__ __forceinline__ void find_border(Want want_of) {
     Border out;
     const u64 s0 = s.sub[2 * lane], s1 = s.sub[2 * lane + 1];
     const uint32_t n0 = s.sub_n[2 * lane], n1 = s.sub_n[2 * lane + 1];
@@ -283,7 +292,8 @@ struct Sampler {
       out.above = __shfl_sync(0xffffffffu, inc, 31);
       out.above_n = (int)__shfl_sync(0xffffffffu, inc_n, 31);
       out.in_n = 0;
-      return out;
+      if (lane == 0) s.border = out;
+      return;
     }
     const int src = __ffs(at) - 1;
     const bool second = before + s0 < out.want;
@@ -302,7 +312,7 @@ struct Sampler {
     out.above = __shfl_sync(0xffffffffu, upto - ba, hit);
     out.above_n = (int)__shfl_sync(0xffffffffu, upto_n - bn, hit);
     out.in_n = (int)__shfl_sync(0xffffffffu, bn, hit);
-    return out;
+    if (lane == 0) s.border = out;
   }
 
   // The n (<= kList) logits that `take` accepts, as (order image, ~index), in
@@ -474,7 +484,7 @@ struct Sampler {
                                    [&](float v) { return bucket(v); }, want_of);
     if (at.in_n == 0) return false;  // fewer logits above -inf than k
     const int n = at.above_n + at.in_n;
-    if (n > kList) {
+    if (n > kFew) {
       cut_in_bucket<MASS>(at.bin, at.want - at.above, at.in_n);
       return false;
     }
@@ -611,24 +621,26 @@ __global__ void __launch_bounds__(kThreads, 2)
     return;
   // The draw by sums: warps take neighbouring segments of the CTA's logits.
   // min-p: logits well above and below its distance need no exponential.
-  const float dist = M > 0.f ? (float)(-log((double)M) * (double)T) : 0.f;
+  const float dist = T == INFINITY ? T : M > 0.f && M < 1.f ? (float)(-log((double)M) * T) : 0.f;
+  auto stays = [&](float v, int i) {
+    if (i >= len || v < a.far || !a.kept(v, begin + i)) return false;
+    const float d = top - v;
+    return M == 0.f || d < dist * 0.99999f || (d <= dist * 1.00001f && !a.below(v, M));
+  };
   auto weight = [&](int i) -> u64 {
-    const float v = i < len ? x[i] : -INFINITY;
-    const u64 w = a.fixed(v);
-    if (M > 0.f) {
-      const float d = top - v;
-      if (d > dist * 1.00001f || (d >= dist * 0.99999f && a.below(v, M))) return 0;
-    }
-    return a.kept(v, begin + i) ? w : 0;
+    const float v = x[min(i, slice - 1)];
+    return stays(v, i) ? a.fixed(v) : 0;
   };
   const int part = (len + kWarps * 128 - 1) / (kWarps * 128) * 128;
   const int w0 = min(warp * part, len), w1 = min(w0 + part, len);
   u64 sum = 0;
   for (int i = w0 + 4 * lane; i < w1; i += 128) {
-    u64 w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = weight(i + e);  // 0 past the part's end
-    sum += (w[0] + w[1]) + (w[2] + w[3]);
+    const float4 v = *reinterpret_cast<const float4*>(x + i);
+    const bool k0 = stays(v.x, i), k1 = stays(v.y, i + 1), k2 = stays(v.z, i + 2),
+               k3 = stays(v.w, i + 3);
+    if (!(k0 || k1 || k2 || k3)) continue;
+    const u64 f0 = a.fixed(v.x), f1 = a.fixed(v.y), f2 = a.fixed(v.z), f3 = a.fixed(v.w);
+    sum += ((k0 ? f0 : 0) + (k1 ? f1 : 0)) + ((k2 ? f2 : 0) + (k3 ? f3 : 0));
   }
   sum = warp_sum(sum);
   __syncthreads();
