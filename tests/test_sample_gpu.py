@@ -35,7 +35,7 @@ def settings_of(rng, rows, k_hi):
 
 
 @pytest.mark.parametrize("vocab", [1, 2, 3, 31, 32, 33, 127, 1000, 4097, 32000, 50257, 128256, 150001])
-@pytest.mark.parametrize("rows", [1, 5])
+@pytest.mark.parametrize("rows", [1, 5, 70])
 def test_random_rows(vocab, rows):
     rng = np.random.default_rng(vocab + rows)
     x = (rng.standard_normal((rows, vocab)) * 3).astype(np.float32)
@@ -80,8 +80,9 @@ def test_a_token_is_hit_in_proportion_to_its_weight():
     assert np.abs(share - np.array([4, 1, 2, 0, 8, 0]) / 15).max() <= 2 / 4096
 
 
-def test_masked_logits():
-    """-inf, NaN, the type's lowest value and rows without anything."""
+@pytest.mark.parametrize("copies", [1, 9])
+def test_masked_logits(copies):
+    """-inf, NaN, the type's lowest value and rows without anything, in a few rows and in many."""
     rng = np.random.default_rng(6)
     x = (rng.standard_normal((8, 700)) * 2).astype(np.float32)
     x[0] = -np.inf
@@ -95,7 +96,9 @@ def test_masked_logits():
     x[7, :699] = np.finfo(np.float32).min
     s = {"temperature": np.full(8, 0.8), "top_k": np.full(8, 650), "top_p": np.full(8, 0.95)}
     for u in (0.0, 0.3, 0.77):
-        got = check(x, np.full(8, u), **s)
+        many = run(np.tile(x, (copies, 1)), np.full(8 * copies, u), **{k: np.tile(v, copies) for k, v in s.items()})
+        assert np.array_equal(many, np.tile(many[:8], copies))
+        got = check(x, np.full(8, u), got=many[:8], **s)
         assert got[0] == got[1] == -1 and got[2] == 0 and got[7] == 699
         assert got[3] % 2 == 1 and got[4] >= 350 and got[6] in (5, 600)
     greedy = run(x, np.full(8, 0.5), temperature=np.zeros(8))
@@ -130,14 +133,26 @@ def test_settings_at_and_past_their_ends():
     assert run(x, [0.5005], temperature=[np.inf])[0] == 450
 
 
-def test_strided_and_unaligned_rows():
+@pytest.mark.parametrize("rows", [7, 80])
+def test_strided_and_unaligned_rows(rows):
     rng = np.random.default_rng(9)
-    big = torch.from_numpy((rng.standard_normal((7, 3010)) * 2).astype(np.float32)).cuda()
+    big = torch.from_numpy((rng.standard_normal((rows, 3010)) * 2).astype(np.float32)).cuda()
     for start, width in ((0, 3010), (1, 3000), (3, 2999), (2, 17)):
         x = big[:, start:start + width]
-        u = rng.random(7)
-        s = settings_of(rng, 7, width // 2)
+        u = rng.random(rows)
+        s = settings_of(rng, rows, width // 2)
         check(x.cpu().numpy(), u, got=run(x, u, **s), **s)
+
+
+def test_one_row_and_many_rows_agree():
+    """A row's token does not depend on how many rows are drawn with it (two forms of the kernel)."""
+    rng = np.random.default_rng(11)
+    x = np.round(rng.standard_normal((90, 20011)) * 3, 1).astype(np.float32)  # with equal logits
+    u, s = rng.random(90), settings_of(rng, 90, 9000)
+    many = run(x, u, **s)
+    few = np.concatenate([run(x[i:i + 9], u[i:i + 9], **{k: v[i:i + 9] for k, v in s.items()})
+                          for i in range(0, 90, 9)])
+    assert np.array_equal(many, few)
 
 
 def test_repeats_bit_for_bit_and_captures():

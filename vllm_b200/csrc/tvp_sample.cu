@@ -38,9 +38,12 @@ constexpr int kCluster = 8;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBuckets = 2048;
-constexpr int kSegment = kBuckets / kCluster;
 constexpr int kBlocks = kBuckets / 32;  // two per lane of a warp
-static_assert(kBlocks == 64 && kSegment <= kThreads, "border() deals them out so");
+static_assert(kBlocks == 64 && kBuckets / kCluster <= kThreads, "border() deals them out so");
+#ifndef TVP_STREAM_ROWS
+#define TVP_STREAM_ROWS 64
+#endif
+constexpr int kStreamRows = TVP_STREAM_ROWS;  // from so many rows on, one CTA takes a row
 constexpr int kList = 512;  // logits of a bucket that CTA 0 takes in
 // Logits at or above the cut that CTA 0 finishes by itself.  Each-with-each takes
 // 2 x 0.7 us for 128 and 2 x 11 us for 512; the sums take some 3 us of passes.
@@ -61,19 +64,20 @@ struct Border {
   u64 above, want;
 };
 
+template <int CL>
 struct alignas(16) Shared {
-  u64 best[kCluster];  // by rank: (order image, ~index) of the largest logit
-  float least[kCluster];
-  u64 amount[kCluster];  // by rank: a sum that the step at hand exchanges
-  int fills[kCluster];
-  u64 ties[kCluster];
-  u64 seg[kSegment];         // this CTA's segment of the cluster's histogram: amounts
-  uint32_t seg_n[kSegment];  // and counts
-  u64 sub[kBlocks];          // every 32 buckets of the cluster's histogram: amounts
-  uint32_t sub_n[kBlocks];   // and counts
+  static constexpr int kSegment = kBuckets / CL;
+  u64 best[CL];  // by rank: (order image, ~index) of the largest logit
+  float least[CL];
+  u64 amount[CL];  // by rank: a sum that the step at hand exchanges
+  int fills[CL];
+  u64 ties[CL];
+  u64 seg[CL > 1 ? kSegment : 1];         // this CTA's segment of the cluster's histogram: amounts
+  uint32_t seg_n[CL > 1 ? kSegment : 1];  // and counts
+  u64 sub[kBlocks];                       // every 32 buckets of the whole histogram: amounts
+  uint32_t sub_n[kBlocks];                // and counts
   u64 warp[kWarps];
   float warp_lo[kWarps];
-  u64 found;
   double pow[256];
   Cut cut;
   Border border;
@@ -133,19 +137,72 @@ __device__ __forceinline__ void shared_add(u64* at, u64 w) {
   if (hi) atomicAdd(p + 1, hi);
 }
 
+template <int CL>
 struct Sampler {
-  cg::cluster_group cluster;
-  Shared& s;
-  const float* x;  // this CTA's logits, NaN as -inf
+  Shared<CL>& s;
+  const float* x;  // this CTA's logits: in shared memory (CL > 1), or the row itself
   unsigned char* scratch;
-  int rank, begin, len;
+  int rank, begin, len, head;  // logits before the first aligned four of x
   int tid, lane, warp;
   float top;    // finite
   float far;    // logits below it have no weight
   double c256;  // 256 log2(e) / T
   float scale;  // buckets per unit of distance
+  bool infinite;  // the row holds +inf: these count as 0, the others as -inf
   bool cutting;  // a filter has cut the row
   Cut cut;
+
+  // The CTAs of a row: barrier, and another one's shared memory.
+  __device__ static void sync() {
+    if (CL > 1)
+      cg::this_cluster().sync();
+    else
+      __syncthreads();
+  }
+  template <typename V>
+  __device__ static V* of_rank(V* place, int r) {
+    return CL > 1 ? cg::this_cluster().map_shared_rank(place, r) : place;
+  }
+
+  // A logit as the sampler takes it: NaN is -inf, -0 is +0.  Shared memory holds
+  // them so.
+  __device__ __forceinline__ float canon(float v) const {
+    if (CL > 1) return v;
+    v = v != v ? -INFINITY : v + 0.f;
+    return !infinite ? v : v == INFINITY ? 0.f : -INFINITY;
+  }
+  __device__ __forceinline__ float at(int i) const { return canon(x[i]); }
+
+  // Calls visit(four logits, index of the first) for the quads [q0, q1) with
+  // q % kThreads == tid, q0 <= q: `step` threads apart, several loads in flight.
+  template <typename Visit>
+  __device__ __forceinline__ void quads(int q0, int q1, int step, Visit visit) const {
+    constexpr int kBatch = CL > 1 ? 1 : 4;
+    const float4* x4 = reinterpret_cast<const float4*>(x + head);
+    for (int q = q0; q < q1; q += kBatch * step) {
+      float4 v[kBatch];
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e)
+        if (q + e * step < q1) v[e] = x4[q + e * step];
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e)
+        if (q + e * step < q1)
+          visit(make_float4(canon(v[e].x), canon(v[e].y), canon(v[e].z), canon(v[e].w)),
+                head + 4 * (q + e * step));
+    }
+  }
+  __device__ __forceinline__ int n_quads() const { return (len - head) / 4; }
+  // All logits of the CTA; the ones around the quads come as a four with -inf.
+  template <typename Visit>
+  __device__ __forceinline__ void each_four(Visit visit) const {
+    const int n4 = n_quads();
+    quads(tid, n4, kThreads, visit);
+    const int tail = len - head - 4 * n4;
+    if (tid < head + tail) {
+      const int i = tid < head ? tid : len - tail + (tid - head);
+      visit(make_float4(at(i), -INFINITY, -INFINITY, -INFINITY), i);
+    }
+  }
 
   // Weight of a logit in 2^-44 of the largest's.  Without branches, so that the
   // chains of several logits overlap.  (An FP32 form that carries the products'
@@ -167,26 +224,12 @@ struct Sampler {
   __device__ __forceinline__ int bucket(float v) const {  // rises as v falls
     return (int)fminf((top - v) * scale, (float)(kBuckets - 1));
   }
-  __device__ __forceinline__ bool kept(float v, int i) const {
-    if (!cutting) return v > -INFINITY;
+  __device__ __forceinline__ bool kept(float v, int i) const {  // with a weight, that is
+    if (v < far) return false;
+    if (!cutting) return true;
     const uint32_t o = order_of(v);
     return o > cut.key || (o == cut.key && i <= cut.last);
   }
-  // Calls visit(logit, index in the CTA's part) for the CTA's logits, four
-  // neighbours of a thread at a time.
-  template <typename Visit>
-  __device__ __forceinline__ void each_logit(Visit visit) const {
-    const int n4 = len / 4;
-    for (int q = tid; q < n4; q += kThreads) {
-      const float4 v = reinterpret_cast<const float4*>(x)[q];
-      visit(v.x, 4 * q);
-      visit(v.y, 4 * q + 1);
-      visit(v.z, 4 * q + 2);
-      visit(v.w, 4 * q + 3);
-    }
-    if (tid < len - 4 * n4) visit(x[4 * n4 + tid], 4 * n4 + tid);
-  }
-
   // Exclusive sum over the block's threads (all must call), and the total.
   __device__ u64 block_scan(u64 v, u64* total) {
     const u64 inc = warp_scan(v, lane);
@@ -205,9 +248,11 @@ struct Sampler {
   // after its reads.
   template <typename V>
   __device__ void share(V* place, V v) {
-    if (tid < kCluster) cluster.map_shared_rank(place, tid)[rank] = v;
-    cluster.sync();
+    if (tid < CL) of_rank(place, tid)[rank] = v;
+    sync();
   }
+
+  static constexpr int kSegment = kBuckets / CL;
 
   // Histogram of the logits that `take` accepts, by `bin` (0 first in falling
   // order), and the bin where the running amount reaches want(total).
@@ -224,60 +269,66 @@ struct Sampler {
       atomicAdd(&hist_n[b], 1u);
       if (MASS) shared_add(&hist[b], w);
     };
-    const int n4 = len / 4;
-    for (int q = tid; q < n4; q += kThreads) {
-      const float4 v = reinterpret_cast<const float4*>(x)[q];
+    each_four([&](const float4& v, int i) {
+      if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) < far) return;
       u64 w[4] = {};
-      if (MASS && fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= far) {
+      if (MASS) {
         w[0] = fixed(v.x);
         w[1] = fixed(v.y);
         w[2] = fixed(v.z);
         w[3] = fixed(v.w);
       }
-      add(v.x, w[0], 4 * q);
-      add(v.y, w[1], 4 * q + 1);
-      add(v.z, w[2], 4 * q + 2);
-      add(v.w, w[3], 4 * q + 3);
-    }
-    if (tid < len - 4 * n4) {
-      const float v = x[4 * n4 + tid];
-      add(v, MASS ? fixed(v) : 0, 4 * n4 + tid);
-    }
-    cluster.sync();
-    // This CTA's segment over all eight, one bucket per thread of 8 warps, and
-    // the sum of each warp's 32 to every CTA.
-    if (tid < kSegment) {
-      const int b = rank * kSegment + tid;
-      uint32_t ns[kCluster];
-      u64 as[kCluster];
+      add(v.x, w[0], i);
+      add(v.y, w[1], i + 1);
+      add(v.z, w[2], i + 2);
+      add(v.w, w[3], i + 3);
+    });
+    sync();
+    if (CL > 1) {
+      // This CTA's segment over all, one bucket per thread of 8 warps, and the
+      // sum of each warp's 32 to every CTA.
+      if (tid < kSegment) {
+        const int b = rank * kSegment + tid;
+        uint32_t ns[CL];
+        u64 as[CL];
 #pragma unroll
-      for (int r = 0; r < kCluster; ++r) {
-        ns[r] = cluster.map_shared_rank(hist_n, r)[b];
-        if (MASS) as[r] = cluster.map_shared_rank(hist, r)[b];
-      }
-      uint32_t n = 0;
-      u64 a = 0;
+        for (int r = 0; r < CL; ++r) {
+          ns[r] = of_rank(hist_n, r)[b];
+          if (MASS) as[r] = of_rank(hist, r)[b];
+        }
+        uint32_t n = 0;
+        u64 a = 0;
 #pragma unroll
-      for (int r = 0; r < kCluster; ++r) {
-        n += ns[r];
-        a += MASS ? as[r] : ns[r];
+        for (int r = 0; r < CL; ++r) {
+          n += ns[r];
+          a += MASS ? as[r] : ns[r];
+        }
+        s.seg[tid] = a;
+        s.seg_n[tid] = n;
+        a = MASS ? warp_sum(a) : 0;
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (lane < CL) {
+          of_rank(s.sub, lane)[rank * (kSegment / 32) + warp] = MASS ? a : n;
+          of_rank(s.sub_n, lane)[rank * (kSegment / 32) + warp] = n;
+        }
       }
-      s.seg[tid] = a;
-      s.seg_n[tid] = n;
-      a = MASS ? warp_sum(a) : 0;
-      n = __reduce_add_sync(0xffffffffu, n);
-      if (lane < kCluster) {
-        cluster.map_shared_rank(s.sub, lane)[rank * (kSegment / 32) + warp] = MASS ? a : n;
-        cluster.map_shared_rank(s.sub_n, lane)[rank * (kSegment / 32) + warp] = n;
+    } else {
+      for (int block = warp; block < kBlocks; block += kWarps) {
+        const uint32_t n = __reduce_add_sync(0xffffffffu, hist_n[block * 32 + lane]);
+        const u64 a = MASS ? warp_sum(hist[block * 32 + lane]) : n;
+        if (lane == 0) {
+          s.sub[block] = a;
+          s.sub_n[block] = n;
+        }
       }
     }
-    cluster.sync();
+    sync();
     // One warp finds the 32 buckets, then the bucket.
-    if (warp == 0) find_border(want_of);
+    if (warp == 0) find_border<MASS>(want_of);
     __syncthreads();
     return s.border;
   }
-  template <typename Want>
+  template <bool MASS, typename Want>
   __device__ __forceinline__ void find_border(Want want_of) {
     Border out;
     const u64 s0 = s.sub[2 * lane], s1 = s.sub[2 * lane + 1];
@@ -301,10 +352,18 @@ struct Sampler {
     const u64 above = __shfl_sync(0xffffffffu, second ? before + s0 : before, src);
     const uint32_t above_n =
         __shfl_sync(0xffffffffu, second ? inc_n - n1 : inc_n - n0 - n1, src);
-    constexpr int kPer = kSegment / 32;  // blocks of a CTA
-    const int place = block % kPer * 32 + lane;
-    const u64 ba = cluster.map_shared_rank(s.seg, block / kPer)[place];
-    const uint32_t bn = cluster.map_shared_rank(s.seg_n, block / kPer)[place];
+    u64 ba;
+    uint32_t bn;
+    if (CL > 1) {
+      constexpr int kPer = kSegment / 32;  // blocks of a CTA
+      const int place = block % kPer * 32 + lane;
+      ba = of_rank(s.seg, block / kPer)[place];
+      bn = of_rank(s.seg_n, block / kPer)[place];
+    } else {
+      const u64* hist = reinterpret_cast<const u64*>(scratch);
+      bn = reinterpret_cast<const uint32_t*>(hist + kBuckets)[block * 32 + lane];
+      ba = MASS ? hist[block * 32 + lane] : bn;
+    }
     const u64 upto = above + warp_scan(ba, lane);
     const uint32_t upto_n = above_n + warp_scan(bn, lane);
     const int hit = __ffs(__ballot_sync(0xffffffffu, upto >= out.want)) - 1;
@@ -324,22 +383,31 @@ struct Sampler {
     u64* mine = reinterpret_cast<u64*>(scratch);
     if (tid == 0) s.fill = 0;
     __syncthreads();
-    each_logit([&](float v, int i) {
+    if (CL == 1) mine = list();
+    auto put = [&](float v, int i) {
       if (take(v, begin + i))
         mine[atomicAdd(&s.fill, 1)] = ((u64)order_of(v) << 32) | (uint32_t)~(begin + i);
+    };
+    each_four([&](const float4& v, int i) {
+      if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) < far) return;
+      put(v.x, i);
+      put(v.y, i + 1);
+      put(v.z, i + 2);
+      put(v.w, i + 3);
     });
     __syncthreads();
+    if (CL == 1) return true;
     share(s.fills, s.fill);
     if (rank != 0) return false;
     if (tid < n) {
-      int r = 0, at = tid;
+      int r = 0, from = tid;
 #pragma unroll
-      for (int q = 0; q < kCluster - 1; ++q)
-        if (r == q && at >= s.fills[q]) {
-          at -= s.fills[q];
+      for (int q = 0; q < CL - 1; ++q)
+        if (r == q && from >= s.fills[q]) {
+          from -= s.fills[q];
           ++r;
         }
-      list()[tid] = cluster.map_shared_rank(mine, r)[at];
+      list()[tid] = of_rank(mine, r)[from];
     }
     __syncthreads();
     return true;
@@ -434,10 +502,10 @@ struct Sampler {
         ahead = over_parts(ahead, sh.parts);
         if (sh.i < in_n && sh.q == 0 && ahead < need && ahead + w[sh.i] >= need) {
           const Cut c = {(uint32_t)(me >> 32), (int)~(uint32_t)me};
-          for (int r = 0; r < kCluster; ++r) *cluster.map_shared_rank(&s.cut, r) = c;
+          for (int r = 0; r < CL; ++r) *of_rank(&s.cut, r) = c;
         }
       }
-      cluster.sync();
+      sync();
       cut = s.cut;
       cutting = true;
       return;
@@ -447,13 +515,13 @@ struct Sampler {
     const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
     for (int d = 0; d < 3; ++d) {
       const uint32_t top_digit = (1u << bits[d]) - 1u;
-      const Border at = border<MASS>(
+      const Border part = border<MASS>(
           [&](float v, int i) { return inside(v, i) && (order_of(v) & mask) == prefix; },
           [&](float v) { return (int)(top_digit - ((order_of(v) >> shifts[d]) & top_digit)); },
           [&](u64) { return left; });
-      prefix |= (top_digit - (uint32_t)at.bin) << shifts[d];
+      prefix |= (top_digit - (uint32_t)part.bin) << shifts[d];
       mask |= top_digit << shifts[d];
-      left = at.want - at.above;
+      left = part.want - part.above;
     }
     // `left` of the amount of equal logits: the n-th of them by index.
     const u64 unit = MASS ? fixed(of_order(prefix)) : 1;
@@ -461,7 +529,7 @@ struct Sampler {
     const int each = (len + kThreads - 1) / kThreads;
     const int i0 = min(tid * each, len), i1 = min(i0 + each, len);
     u64 ties = 0, all;
-    for (int i = i0; i < i1; ++i) ties += kept(x[i], begin + i) && order_of(x[i]) == prefix;
+    for (int i = i0; i < i1; ++i) ties += kept(at(i), begin + i) && order_of(at(i)) == prefix;
     const u64 before = block_scan(ties, &all);
     share(s.ties, all);
     u64 seen = before;
@@ -469,10 +537,10 @@ struct Sampler {
     int last = -1;
     if (seen < nth && seen + ties >= nth)
       for (int i = i0; i < i1; ++i)
-        if (kept(x[i], begin + i) && order_of(x[i]) == prefix && ++seen == nth) last = begin + i;
+        if (kept(at(i), begin + i) && order_of(at(i)) == prefix && ++seen == nth) last = begin + i;
     if (last >= 0)
-      for (int r = 0; r < kCluster; ++r) *cluster.map_shared_rank(&s.cut, r) = {prefix, last};
-    cluster.sync();
+      for (int r = 0; r < CL; ++r) *of_rank(&s.cut, r) = {prefix, last};
+    sync();
     cut = s.cut;
     cutting = true;
   }
@@ -480,85 +548,83 @@ struct Sampler {
   // One filter: true when it ended the row (the token is written).
   template <bool MASS, typename Want>
   __device__ bool filter(Want want_of, int k, float P, float M, float u, int32_t* token) {
-    const Border at = border<MASS>([&](float v, int i) { return kept(v, i); },
+    const Border edge = border<MASS>([&](float v, int i) { return kept(v, i); },
                                    [&](float v) { return bucket(v); }, want_of);
-    if (at.in_n == 0) return false;  // fewer logits above -inf than k
-    const int n = at.above_n + at.in_n;
+    if (edge.in_n == 0) return false;  // fewer logits with a weight than k
+    const int n = edge.above_n + edge.in_n;
     if (n > kFew) {
-      cut_in_bucket<MASS>(at.bin, at.want - at.above, at.in_n);
+      cut_in_bucket<MASS>(edge.bin, edge.want - edge.above, edge.in_n);
       return false;
     }
     // After a histogram of weights the amount wanted is known, of the whole;
     // after one of counts, top-p is of the k that are left.
-    if (gather([&](float v, int i) { return bucket(v) <= at.bin && kept(v, i); }, n))
-      finish(n, MASS ? 0 : k, MASS ? at.want : 0, P, M, u, token);
-    cluster.sync();  // CTA 0 reads the others' lists
+    if (gather([&](float v, int i) { return bucket(v) <= edge.bin && kept(v, i); }, n))
+      finish(n, MASS ? 0 : k, MASS ? edge.want : 0, P, M, u, token);
+    sync();  // CTA 0 reads the others' lists
     return true;
   }
 };
 
+template <int CL>
 __global__ void __launch_bounds__(kThreads, 2)
     sample_kernel(const float* __restrict__ logits, int vocab, int slice, long long row_stride,
                   const float* __restrict__ uniforms, const float* __restrict__ temperature,
                   const int32_t* __restrict__ top_k, const float* __restrict__ top_p,
                   const float* __restrict__ min_p, int32_t* __restrict__ tokens) {
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ Shared s;
-  const cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), row = blockIdx.x / kCluster;
+  __shared__ Shared<CL> s;
+  const int rank = CL > 1 ? (int)cg::this_cluster().block_rank() : 0, row = blockIdx.x / CL;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int begin = min(rank * slice, vocab), len = min(slice, vocab - begin);
-  float* x = reinterpret_cast<float*>(smem + kScratchBytes);
+  const float* src = logits + (size_t)row * row_stride + begin;
+  // Logits before the first 16-byte boundary.
+  const int head = min((int)((0u - (uint32_t)(reinterpret_cast<uintptr_t>(src) >> 2)) & 3u), len);
+  float* x = reinterpret_cast<float*>(smem + kScratchBytes);  // CL > 1
 
-  // This CTA's logits into shared memory, and the row's largest and least.
+  // The row's largest and least logit; with CL > 1 the CTA's logits also go into
+  // shared memory.
   float hi = -INFINITY, lo = INFINITY;
   int hi_at = 0;
-  auto put = [&](float v, int i) -> float {
+  auto see = [&](float v, int i) {
     v = v != v ? -INFINITY : v + 0.f;  // -0 is +0
-    if (v > hi) {  // indices rise within a thread: the lowest of equals stays
+    if (v > hi || (v == hi && begin + i < hi_at)) {
       hi = v;
       hi_at = begin + i;
     }
     if (v > -INFINITY) lo = fminf(lo, v);
     return v;
   };
-  const float* src = logits + (size_t)row * row_stride + begin;
-  int done = 0;
-  if ((reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
-    const int n4 = len / 4;
-    constexpr int kBatch = 8;
-    for (int base = tid; base < n4; base += kBatch * kThreads) {
-      float4 v[kBatch];
+  const int n4 = (len - head) / 4;
+  constexpr int kBatch = 8;
+  for (int base = tid; base < n4; base += kBatch * kThreads) {
+    float4 v[kBatch];
 #pragma unroll
-      for (int e = 0; e < kBatch; ++e)
-        if (base + e * kThreads < n4)
-          v[e] = __ldcs(reinterpret_cast<const float4*>(src) + base + e * kThreads);
+    for (int e = 0; e < kBatch; ++e)
+      if (base + e * kThreads < n4)
+        v[e] = __ldg(reinterpret_cast<const float4*>(src + head) + base + e * kThreads);
 #pragma unroll
-      for (int e = 0; e < kBatch; ++e) {
-        const int q = base + e * kThreads;
-        if (q >= n4) break;
-        float4 w;
-        w.x = put(v[e].x, 4 * q);
-        w.y = put(v[e].y, 4 * q + 1);
-        w.z = put(v[e].z, 4 * q + 2);
-        w.w = put(v[e].w, 4 * q + 3);
-        reinterpret_cast<float4*>(x)[q] = w;
+    for (int e = 0; e < kBatch; ++e) {
+      const int i = head + 4 * (base + e * kThreads);
+      if (base + e * kThreads >= n4) break;
+      const float4 c = make_float4(see(v[e].x, i), see(v[e].y, i + 1), see(v[e].z, i + 2),
+                                   see(v[e].w, i + 3));
+      if (CL > 1) {
+        if (head == 0) {
+          *reinterpret_cast<float4*>(x + i) = c;
+        } else {
+          x[i] = c.x;
+          x[i + 1] = c.y;
+          x[i + 2] = c.z;
+          x[i + 3] = c.w;
+        }
       }
     }
-    done = n4 * 4;
   }
-  constexpr int kBatch1 = 16;
-  for (int base = done + tid; base < len; base += kBatch1 * kThreads) {
-    float v[kBatch1];
-#pragma unroll
-    for (int e = 0; e < kBatch1; ++e)
-      if (base + e * kThreads < len) v[e] = __ldcs(src + base + e * kThreads);
-#pragma unroll
-    for (int e = 0; e < kBatch1; ++e) {
-      const int i = base + e * kThreads;
-      if (i >= len) break;
-      x[i] = put(v[e], i);
-    }
+  const int tail = len - head - 4 * n4;
+  if (tid < head + tail) {
+    const int i = tid < head ? tid : len - tail + (tid - head);
+    const float c = see(src[i], i);
+    if (CL > 1) x[i] = c;
   }
   u64 best = hi > -INFINITY ? ((u64)order_of(hi) << 32) | (uint32_t)~hi_at : 0;
 #pragma unroll
@@ -580,19 +646,19 @@ __global__ void __launch_bounds__(kThreads, 2)
   const float M = mp > 0.f ? fminf(mp, 1.f) : 0.f;
   const float u = uniforms[row];
   __syncthreads();
-  if (tid < kCluster) {
+  if (tid < CL) {
     for (int w = 0; w < kWarps; ++w) {
       best = s.warp[w] > best ? s.warp[w] : best;
       lo = fminf(lo, s.warp_lo[w]);
     }
-    cluster.map_shared_rank(s.best, tid)[rank] = best;
-    cluster.map_shared_rank(s.least, tid)[rank] = lo;
+    Sampler<CL>::of_rank(s.best, tid)[rank] = best;
+    Sampler<CL>::of_rank(s.least, tid)[rank] = lo;
   }
-  cluster.sync();
+  Sampler<CL>::sync();
   best = s.best[0];
   lo = s.least[0];
 #pragma unroll
-  for (int r = 1; r < kCluster; ++r) {
+  for (int r = 1; r < CL; ++r) {
     best = s.best[r] > best ? s.best[r] : best;
     lo = fminf(lo, s.least[r]);
   }
@@ -601,47 +667,55 @@ __global__ void __launch_bounds__(kThreads, 2)
     return;
   }
   float top = of_order((uint32_t)(best >> 32));
-  if (top == INFINITY) {  // these share the mass: zeros among -inf
-    for (int i = tid; i < len; i += kThreads) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
+  const bool infinite = top == INFINITY;
+  if (infinite) {  // these share the mass: zeros among -inf
+    if (CL > 1)
+      for (int i = tid; i < len; i += kThreads) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
     __syncthreads();
     top = lo = 0.f;
   }
   // Buckets over the distances that have weight, or over the row's own range
   // where that is narrower.
   const float range = fminf(kFar * T, top - lo);
-  const double c256 = 369.3299304675746 / (double)T;
-  Sampler a = {cluster, s, x, smem, rank, begin, len, tid, lane, warp, top,
-               fmaxf(top - kFar * T, -FLT_MAX), c256,
-               range > 0.f ? (float)kBuckets / range : 0.f, false, {}};
+  Sampler<CL> a = {s, CL > 1 ? x : src, smem, rank, begin, len, CL > 1 ? 0 : head, tid, lane, warp,
+                   top, fmaxf(top - kFar * T, -FLT_MAX), 369.3299304675746 / (double)T,
+                   range > 0.f ? (float)kBuckets / range : 0.f, infinite, false, {}};
   if (k > 0 && k < vocab &&
-      a.filter<false>([&](u64) { return (u64)k; }, k, P, M, u, tokens + row))
+      a.template filter<false>([&](u64) { return (u64)k; }, k, P, M, u, tokens + row))
     return;
-  if (P < 1.f && a.filter<true>([&](u64 total) { return Sampler::want_of(P, total); }, k, P, M, u,
-                                tokens + row))
+  if (P < 1.f &&
+      a.template filter<true>([&](u64 total) { return Sampler<CL>::want_of(P, total); }, k, P, M, u,
+                              tokens + row))
     return;
-  // The draw by sums: warps take neighbouring segments of the CTA's logits.
+  // The draw by sums: warps take neighbouring segments of the CTA's quads, the
+  // first one also what comes before them, the last one what comes after.
   // min-p: logits well above and below its distance need no exponential.
   const float dist = T == INFINITY ? T : M > 0.f && M < 1.f ? (float)(-log((double)M) * T) : 0.f;
   auto stays = [&](float v, int i) {
-    if (i >= len || v < a.far || !a.kept(v, begin + i)) return false;
+    if (!a.kept(v, begin + i)) return false;
     const float d = top - v;
     return M == 0.f || d < dist * 0.99999f || (d <= dist * 1.00001f && !a.below(v, M));
   };
   auto weight = [&](int i) -> u64 {
-    const float v = x[min(i, slice - 1)];
+    const float v = a.at(i);
     return stays(v, i) ? a.fixed(v) : 0;
   };
-  const int part = (len + kWarps * 128 - 1) / (kWarps * 128) * 128;
-  const int w0 = min(warp * part, len), w1 = min(w0 + part, len);
+  const int all = a.n_quads(), part = (all + kWarps * 32 - 1) / (kWarps * 32) * 32;
   u64 sum = 0;
-  for (int i = w0 + 4 * lane; i < w1; i += 128) {
-    const float4 v = *reinterpret_cast<const float4*>(x + i);
+  a.quads(warp * part + lane, min((warp + 1) * part, all), 32, [&](const float4& v, int i) {
     const bool k0 = stays(v.x, i), k1 = stays(v.y, i + 1), k2 = stays(v.z, i + 2),
                k3 = stays(v.w, i + 3);
-    if (!(k0 || k1 || k2 || k3)) continue;
+    if (!(k0 || k1 || k2 || k3)) return;
     const u64 f0 = a.fixed(v.x), f1 = a.fixed(v.y), f2 = a.fixed(v.z), f3 = a.fixed(v.w);
     sum += ((k0 ? f0 : 0) + (k1 ? f1 : 0)) + ((k2 ? f2 : 0) + (k3 ? f3 : 0));
-  }
+  });
+  // Where segment w of the CTA starts.
+  auto start_of = [&](int w) {
+    return w == 0 ? 0 : w == kWarps ? len : a.head + 4 * min(w * part, all);
+  };
+  if (warp == 0 && lane < a.head) sum += weight(lane);
+  const int after = a.head + 4 * all;
+  if (warp == kWarps - 1 && lane < len - after) sum += weight(after + lane);
   sum = warp_sum(sum);
   __syncthreads();
   if (lane == 0) s.warp[warp] = sum;
@@ -651,16 +725,16 @@ __global__ void __launch_bounds__(kThreads, 2)
   a.share(s.amount, mine);
   u64 total = 0, before = 0;
 #pragma unroll
-  for (int r = 0; r < kCluster; ++r) {
+  for (int r = 0; r < CL; ++r) {
     if (r < rank) before += s.amount[r];
     total += s.amount[r];
   }
-  const u64 point = Sampler::point_of(u, total);
+  const u64 point = Sampler<CL>::point_of(u, total);
   if (before > point || before + mine <= point) return;
   // The whole CTA goes over the segment that holds the point.
   int seg = 0;
   while (before + s.warp[seg] <= point) before += s.warp[seg++];
-  const int s0 = min(seg * part, len), s1 = min(s0 + part, len);
+  const int s0 = start_of(seg), s1 = start_of(seg + 1);
   const int each = (s1 - s0 + kThreads - 1) / kThreads;
   const int i0 = min(s0 + tid * each, s1), i1 = min(i0 + each, s1);
   mine = 0;
@@ -679,6 +753,43 @@ __global__ void __launch_bounds__(kThreads, 2)
 
 using namespace tvp;
 
+namespace {
+
+template <int CL>
+cudaError_t launch_sampler(int rows, int vocab, long long row_stride, const float* logits,
+                           const float* uniforms, const float* temperature, const int32_t* top_k,
+                           const float* top_p, const float* min_p, int32_t* tokens,
+                           cudaStream_t stream) {
+  auto slice_of = [](int v) { return CL > 1 ? ((v + CL - 1) / CL + 3) / 4 * 4 : v; };
+  auto smem_of = [](int slice) { return kScratchBytes + (CL > 1 ? (size_t)slice * 4 : 0); };
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    e = cudaFuncSetAttribute(sample_kernel<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)smem_of(slice_of(TVP_SAMPLE_MAX_VOCAB)));
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  const int slice = slice_of(vocab);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows * CL);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem_of(slice);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CL;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<CL>, logits, vocab, slice, row_stride, uniforms,
+                            temperature, top_k, top_p, min_p, tokens);
+}
+
+}  // namespace
+
 extern "C" int tvp_sample_tokens(const float* d_logits, int rows, int vocab, long long row_stride,
                                  const float* d_uniforms, const float* d_temperature,
                                  const int32_t* d_top_k, const float* d_top_p, const float* d_min_p,
@@ -687,31 +798,12 @@ extern "C" int tvp_sample_tokens(const float* d_logits, int rows, int vocab, lon
       (reinterpret_cast<uintptr_t>(d_logits) & 3u))
     return TVP_ERR_INVALID_ARGUMENT;
   if (vocab > TVP_SAMPLE_MAX_VOCAB || rows > 65535) return TVP_ERR_UNSUPPORTED;
-  auto slice_of = [](int v) { return ((v + kCluster - 1) / kCluster + 3) / 4 * 4; };
-  static bool configured[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return TVP_ERR_RUNTIME;
-  if (dev < 0 || dev >= 64 || !configured[dev]) {
-    if (cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)(kScratchBytes + (size_t)slice_of(TVP_SAMPLE_MAX_VOCAB) * 4)) !=
-        cudaSuccess)
-      return TVP_ERR_RUNTIME;
-    if (dev >= 0 && dev < 64) configured[dev] = true;
-  }
-  const int slice = slice_of(vocab);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)rows * kCluster);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kScratchBytes + (size_t)slice * 4;
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel, d_logits, vocab, slice, row_stride, d_uniforms,
-                            d_temperature, d_top_k, d_top_p, d_min_p, d_tokens) == cudaSuccess
-             ? TVP_OK
-             : TVP_ERR_RUNTIME;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e =
+      rows < kStreamRows
+          ? launch_sampler<kCluster>(rows, vocab, row_stride, d_logits, d_uniforms, d_temperature,
+                                     d_top_k, d_top_p, d_min_p, d_tokens, st)
+          : launch_sampler<1>(rows, vocab, row_stride, d_logits, d_uniforms, d_temperature, d_top_k,
+                              d_top_p, d_min_p, d_tokens, st);
+  return e == cudaSuccess ? TVP_OK : TVP_ERR_RUNTIME;
 }
