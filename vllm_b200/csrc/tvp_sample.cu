@@ -23,6 +23,7 @@
 // count of equal logits by index), and the draw goes by sums: per CTA, per warp,
 // then within the warp's segment in index order.
 #include <cfloat>
+#include <climits>
 
 #include <cooperative_groups.h>
 
@@ -38,19 +39,26 @@ constexpr int kCluster = 8;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBuckets = 2048;
+constexpr int kQuads = 8;  // fours of logits per batch of a thread
 constexpr int kBlocks = kBuckets / 32;  // two per lane of a warp
-static_assert(kBlocks == 64 && kBuckets / kCluster <= kThreads, "border() deals them out so");
-#ifndef TVP_STREAM_ROWS
-#define TVP_STREAM_ROWS 64
-#endif
-constexpr int kStreamRows = TVP_STREAM_ROWS;  // from so many rows on, one CTA takes a row
+static_assert(kBlocks == 64 && kBuckets / kCluster % 32 == 0, "border() deals them out so");
+// Few rows: 8 CTAs keep a row in shared memory.  From kStreamRows on, 4 CTAs per
+// row read it again from L2 (kStreamMany: 2), which leaves room for more rows at
+// once.  Measured, us for rows of 128256 of mixed settings, 8 kept / 4 / 2
+// streaming: 32 rows 32 / 49 / 84, 64 rows 50 / 55 / 85, 96 rows 69 / 64 / 79,
+// 256 rows 157 / 127 / 127, 512 rows 294 / 218 / 194; of top-k 50: 32 rows
+// 14 / 14 / 17, 64 rows 26 / 17 / 17, 256 rows 102 / 67 / 49.
+constexpr int kStreamRows = 64;
+constexpr int kStreamMany = 192;
 constexpr int kList = 512;  // logits of a bucket that CTA 0 takes in
 // Logits at or above the cut that CTA 0 finishes by itself.  Each-with-each takes
 // 2 x 0.7 us for 128 and 2 x 11 us for 512; the sums take some 3 us of passes.
 constexpr int kFew = 160;
 constexpr int kFixedBits = 44;
-// Distances (in units of T) past which a weight rounds to 0: 45 ln 2.
-constexpr float kFar = 31.25f;
+// A distance (in units of T) where a weight rounds to 0: 45 ln 2 is 31.2, and
+// the subtraction's rounding takes half a last place of the top.
+constexpr float kFar = 33.f;
+constexpr double kTwo52 = 4503599627370496.0;
 
 struct Cut {
   uint32_t key;  // kept: order image above it, or equal and index <= last
@@ -67,8 +75,8 @@ struct Border {
 template <int CL>
 struct alignas(16) Shared {
   static constexpr int kSegment = kBuckets / CL;
-  u64 best[CL];  // by rank: (order image, ~index) of the largest logit
-  float least[CL];
+  float most[CL], least[CL];  // by rank: largest and least logit
+  int where[CL];              // by rank: the lowest index of the largest
   u64 amount[CL];  // by rank: a sum that the step at hand exchanges
   int fills[CL];
   u64 ties[CL];
@@ -77,11 +85,13 @@ struct alignas(16) Shared {
   u64 sub[kBlocks];                       // every 32 buckets of the whole histogram: amounts
   uint32_t sub_n[kBlocks];                // and counts
   u64 warp[kWarps];
-  float warp_lo[kWarps];
+  float warp_most[kWarps], warp_least[kWarps];
   double pow[256];
   Cut cut;
   Border border;
   int fill;
+  int part;  // where the draw's point lies, and the sum before
+  u64 run;
 };
 
 // 2^(-j / 256), by the Taylor series of the exponential.
@@ -103,6 +113,11 @@ __device__ const Powers g_powers = Powers();
 
 constexpr size_t kScratchBytes = kBuckets * 12;  // histogram, then the lists
 static_assert(kScratchBytes >= 3 * kList * 8, "the lists fit the histogram's place");
+static_assert(kScratchBytes >= (TVP_SAMPLE_MAX_VOCAB / 128 + 3) * 8, "and so do the sums");
+
+__host__ __device__ constexpr int batches_of(int logits) {
+  return (logits / 4 + kQuads * kThreads - 1) / (kQuads * kThreads);
+}
 
 __device__ __forceinline__ uint32_t order_of(float x) {  // larger logit, larger image
   const uint32_t u = __float_as_uint(x);
@@ -137,16 +152,18 @@ __device__ __forceinline__ void shared_add(u64* at, u64 w) {
   if (hi) atomicAdd(p + 1, hi);
 }
 
-template <int CL>
+template <int CL, bool RES>
 struct Sampler {
   Shared<CL>& s;
-  const float* x;  // this CTA's logits: in shared memory (CL > 1), or the row itself
+  const float* x;  // this CTA's logits: in shared memory (RES), or the row itself
+  const float* maxima;  // of each thread's batches
   unsigned char* scratch;
   int rank, begin, len, head;  // logits before the first aligned four of x
   int tid, lane, warp;
   float top;    // finite
-  float far;    // logits below it have no weight
+  float far;    // logits at and below it have no weight
   double c256;  // 256 log2(e) / T
+  double reach_p;  // min-p keeps the logits up to this far below the top
   float scale;  // buckets per unit of distance
   bool infinite;  // the row holds +inf: these count as 0, the others as -inf
   bool cutting;  // a filter has cut the row
@@ -164,62 +181,103 @@ struct Sampler {
     return CL > 1 ? cg::this_cluster().map_shared_rank(place, r) : place;
   }
 
-  // A logit as the sampler takes it: NaN is -inf, -0 is +0.  Shared memory holds
-  // them so.
-  __device__ __forceinline__ float canon(float v) const {
-    if (CL > 1) return v;
-    v = v != v ? -INFINITY : v + 0.f;
-    return !infinite ? v : v == INFINITY ? 0.f : -INFINITY;
+  // A logit as the sampler takes it: NaN is -inf, -0 is +0; in a row with +inf
+  // these count as 0, the others as -inf.  Shared memory holds them so.
+  __device__ __forceinline__ static float canon(float v) { return fmaxf(v + 0.f, -INFINITY); }
+  __device__ __forceinline__ static float only(float v) { return v == INFINITY ? 0.f : -INFINITY; }
+  __device__ __forceinline__ float at(int i) const {
+    if (RES) return x[i];
+    return infinite ? only(x[i]) : canon(x[i]);
   }
-  __device__ __forceinline__ float at(int i) const { return canon(x[i]); }
 
-  // Calls visit(four logits, index of the first) for the quads [q0, q1) with
-  // q % kThreads == tid, q0 <= q: `step` threads apart, several loads in flight.
-  template <typename Visit>
-  __device__ __forceinline__ void quads(int q0, int q1, int step, Visit visit) const {
-    constexpr int kBatch = CL > 1 ? 1 : 4;
-    const float4* x4 = reinterpret_cast<const float4*>(x + head);
-    for (int q = q0; q < q1; q += kBatch * step) {
-      float4 v[kBatch];
-#pragma unroll
-      for (int e = 0; e < kBatch; ++e)
-        if (q + e * step < q1) v[e] = x4[q + e * step];
-#pragma unroll
-      for (int e = 0; e < kBatch; ++e)
-        if (q + e * step < q1)
-          visit(make_float4(canon(v[e].x), canon(v[e].y), canon(v[e].z), canon(v[e].w)),
-                head + 4 * (q + e * step));
-    }
-  }
+  // A thread's batch `it` is the kQuads quads of logits (it kQuads + e) kThreads +
+  // tid after the head: a warp's quads of one e are 128 neighbouring logits.
   __device__ __forceinline__ int n_quads() const { return (len - head) / 4; }
-  // All logits of the CTA; the ones around the quads come as a four with -inf.
-  template <typename Visit>
-  __device__ __forceinline__ void each_four(Visit visit) const {
+  __device__ __forceinline__ int n_batches() const {
+    return (n_quads() + kQuads * kThreads - 1) / (kQuads * kThreads);
+  }
+  // Quads e0 .. e0 + 3 of batch `it`, -inf past the last one, as they are stored
+  // or as the sampler takes them.
+  template <bool RAW = false>
+  __device__ __forceinline__ void half_batch(int it, int e0, float4 (&v)[4]) const {
+    const float4* x4 = reinterpret_cast<const float4*>(x + head);
     const int n4 = n_quads();
-    quads(tid, n4, kThreads, visit);
-    const int tail = len - head - 4 * n4;
-    if (tid < head + tail) {
-      const int i = tid < head ? tid : len - tail + (tid - head);
-      visit(make_float4(at(i), -INFINITY, -INFINITY, -INFINITY), i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int q = (it * kQuads + e0 + e) * kThreads + tid;
+      v[e] = q < n4 ? x4[q] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    }
+    if (RES || RAW) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      v[e] = make_float4(canon(v[e].x), canon(v[e].y), canon(v[e].z), canon(v[e].w));
+    if (infinite) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[e] = make_float4(only(v[e].x), only(v[e].y), only(v[e].z), only(v[e].w));
     }
   }
+  // Index of the first logit of quad e of batch `it`.
+  __device__ __forceinline__ int place(int it, int e) const {
+    return head + 4 * ((it * kQuads + e) * kThreads + tid);
+  }
+  // Calls visit(four logits, index of the first) for the CTA's logits; batches
+  // whose largest is below `least` are left out.  The logits around the quads
+  // come as fours with -inf.
+  template <typename Visit>
+  __device__ __forceinline__ void each_four(float least, Visit visit) const {
+    const int n = n_batches();
+    for (int it = 0; it < n; ++it) {
+      if (maxima[it * kThreads + tid] < least) continue;
+#pragma unroll 1  // the code of a pass is fetched once per row: it had better be short
+      for (int e0 = 0; e0 < kQuads; e0 += 4) {
+        float4 v[4];
+        half_batch(it, e0, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (fmaxf(fmaxf(v[e].x, v[e].y), fmaxf(v[e].z, v[e].w)) >= least)
+            visit(v[e], place(it, e0 + e));
+      }
+    }
+    const int i = single();
+    if (i >= 0) visit(make_float4(at(i), -INFINITY, -INFINITY, -INFINITY), i);
+  }
+  // This thread's logit among the up to 6 before and after the quads, or -1.
+  __device__ __forceinline__ int single() const {
+    const int tail = (len - head) & 3;
+    return tid < head ? tid : tid < head + tail ? len - tail + (tid - head) : -1;
+  }
+  // No kept logit is below this.
+  __device__ __forceinline__ float least_kept() const {
+    return cutting ? fmaxf(far, of_order(cut.key)) : far;
+  }
 
-  // Weight of a logit in 2^-44 of the largest's.  Without branches, so that the
-  // chains of several logits overlap.  (An FP32 form that carries the products'
-  // rounding errors along, good to 2^-31, measured the same time: 11 FP64
-  // instructions against some 30 FP32 ones.)
-  __device__ __forceinline__ u64 fixed(float v) const {
+  // 2^52 + the weight of a logit in 2^-44 of the largest's: the sum's mantissa
+  // holds the integer.  Without branches, so that the chains of several logits
+  // overlap; a logit below `far`, a NaN among them, counts as `far`, which rounds
+  // to 0.  (The passes that weigh every logit are bound by instruction issue:
+  // 67 per 32 logits, with masks and selects, took 77 us for 256 rows of 128256.)
+  __device__ __forceinline__ double weigh(float v) const {
     const double t = ((double)top - (double)fmaxf(v, far)) * c256;
     const double shifted = t + 6755399441055744.0;  // 1.5 * 2^52: rounds to an integer
     const int k = __double2loint(shifted);
-    const double f = ((shifted - 6755399441055744.0) - t) * (0.6931471805599453 / 256);
-    double y = fma(f, 1.0 / 6.0, 0.5);
+    const double f = (shifted - 6755399441055744.0) - t;
+    constexpr double kStep = 0.6931471805599453 / 256;  // ln 2 per 256th of an octave
+    double y = fma(f, kStep * kStep * kStep / 6, kStep * kStep / 2);
+    y = fma(y, f, kStep);
     y = fma(y, f, 1.0);
-    y = fma(y, f, 1.0);
-    y *= s.pow[k & 255];
-    // * 2^(44 - k / 256), then the integer part from the sum's mantissa
-    y = fma(y, __hiloint2double((1023 + kFixedBits - (k >> 8)) << 20, 0), 4503599627370496.0);
-    return v < far ? 0ull : (u64)__double_as_longlong(y) & 0xfffffffffffffull;
+    const double p = s.pow[k & 255];  // * 2^(44 - k / 256)
+    const double scaled = __hiloint2double(
+        __double2hiint(p) + (kFixedBits << 20) - ((k & ~255) << 12), __double2loint(p));
+    return fma(y, scaled, kTwo52);
+  }
+  __device__ __forceinline__ u64 fixed(float v) const {
+    return (u64)__double_as_longlong(weigh(v)) & 0xfffffffffffffull;
+  }
+  // The sum of four, exact in FP64.
+  __device__ __forceinline__ double weigh4(const float4& v) const {
+    return ((weigh(v.x) - kTwo52) + (weigh(v.y) - kTwo52)) +
+           ((weigh(v.z) - kTwo52) + (weigh(v.w) - kTwo52));
   }
   __device__ __forceinline__ int bucket(float v) const {  // rises as v falls
     return (int)fminf((top - v) * scale, (float)(kBuckets - 1));
@@ -254,9 +312,10 @@ struct Sampler {
 
   static constexpr int kSegment = kBuckets / CL;
 
-  // Histogram of the logits that `take` accepts, by `bin` (0 first in falling
-  // order), and the bin where the running amount reaches want(total).
-  template <bool MASS, typename Take, typename Bin, typename Want>
+  // Histogram of the kept logits that `take` accepts, by `bin` (0 first in
+  // falling order), and the bin where the running amount reaches want(total).
+  // With MAXIMA: of the batches' largest logits, each counted once.
+  template <bool MASS, bool MAXIMA, typename Take, typename Bin, typename Want>
   __device__ Border border(Take take, Bin bin, Want want_of) {
     u64* hist = reinterpret_cast<u64*>(scratch);
     uint32_t* hist_n = reinterpret_cast<uint32_t*>(hist + kBuckets);
@@ -264,31 +323,40 @@ struct Sampler {
       reinterpret_cast<uint4*>(scratch)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     auto add = [&](float v, u64 w, int i) {
-      if (!take(v, begin + i)) return;
+      if (!kept(v, begin + i) || !take(v)) return;
       const int b = bin(v);
       atomicAdd(&hist_n[b], 1u);
       if (MASS) shared_add(&hist[b], w);
     };
-    each_four([&](const float4& v, int i) {
-      if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) < far) return;
-      u64 w[4] = {};
-      if (MASS) {
-        w[0] = fixed(v.x);
-        w[1] = fixed(v.y);
-        w[2] = fixed(v.z);
-        w[3] = fixed(v.w);
+    if (MAXIMA) {
+      const int n = n_batches();
+      for (int it = 0; it < n; ++it) {
+        const float v = maxima[it * kThreads + tid];
+        if (v >= far) atomicAdd(&hist_n[bin(v)], 1u);
       }
-      add(v.x, w[0], i);
-      add(v.y, w[1], i + 1);
-      add(v.z, w[2], i + 2);
-      add(v.w, w[3], i + 3);
-    });
+      const int i = single();
+      if (i >= 0) add(at(i), 0, i);
+    } else {
+      each_four(least_kept(), [&](const float4& v, int i) {
+        u64 w[4] = {};
+        if (MASS) {
+          w[0] = fixed(v.x);
+          w[1] = fixed(v.y);
+          w[2] = fixed(v.z);
+          w[3] = fixed(v.w);
+        }
+        add(v.x, w[0], i);
+        add(v.y, w[1], i + 1);
+        add(v.z, w[2], i + 2);
+        add(v.w, w[3], i + 3);
+      });
+    }
     sync();
     if (CL > 1) {
-      // This CTA's segment over all, one bucket per thread of 8 warps, and the
-      // sum of each warp's 32 to every CTA.
-      if (tid < kSegment) {
-        const int b = rank * kSegment + tid;
+      // This CTA's segment over all, and the sum of each warp's 32 buckets to
+      // every CTA.
+      for (int i = tid; i < kSegment; i += kThreads) {
+        const int b = rank * kSegment + i;
         uint32_t ns[CL];
         u64 as[CL];
 #pragma unroll
@@ -303,13 +371,13 @@ struct Sampler {
           n += ns[r];
           a += MASS ? as[r] : ns[r];
         }
-        s.seg[tid] = a;
-        s.seg_n[tid] = n;
+        s.seg[i] = a;
+        s.seg_n[i] = n;
         a = MASS ? warp_sum(a) : 0;
         n = __reduce_add_sync(0xffffffffu, n);
         if (lane < CL) {
-          of_rank(s.sub, lane)[rank * (kSegment / 32) + warp] = MASS ? a : n;
-          of_rank(s.sub_n, lane)[rank * (kSegment / 32) + warp] = n;
+          of_rank(s.sub, lane)[b / 32] = MASS ? a : n;
+          of_rank(s.sub_n, lane)[b / 32] = n;
         }
       }
     } else {
@@ -374,43 +442,50 @@ struct Sampler {
     if (lane == 0) s.border = out;
   }
 
-  // The n (<= kList) logits that `take` accepts, as (order image, ~index), in
-  // CTA 0's list, in no order.  Only CTA 0 returns true.
+  // The kept logits in buckets first .. last, as (order image, ~index), in CTA
+  // 0's list, in no order; returns how many there are in the row.  More than
+  // `most` (<= kList) are not listed.
   __device__ u64* list() const { return reinterpret_cast<u64*>(scratch) + kList; }
   __device__ u64* weights() const { return reinterpret_cast<u64*>(scratch) + 2 * kList; }
-  template <typename Take>
-  __device__ bool gather(Take take, int n) {
-    u64* mine = reinterpret_cast<u64*>(scratch);
+  __device__ int gather(int first, int last, int most) {
+    u64* mine = CL == 1 ? list() : reinterpret_cast<u64*>(scratch);
     if (tid == 0) s.fill = 0;
     __syncthreads();
-    if (CL == 1) mine = list();
     auto put = [&](float v, int i) {
-      if (take(v, begin + i))
-        mine[atomicAdd(&s.fill, 1)] = ((u64)order_of(v) << 32) | (uint32_t)~(begin + i);
+      if (!kept(v, begin + i) || bucket(v) < first || bucket(v) > last) return;
+      const int to = atomicAdd(&s.fill, 1);
+      if (to < most) mine[to] = ((u64)order_of(v) << 32) | (uint32_t)~(begin + i);
     };
-    each_four([&](const float4& v, int i) {
-      if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) < far) return;
+    // A logit of bucket `last` lies above this (the distance is rounded, by 2^-23
+    // of it at most, and so are the product and the quotient).
+    const float reach =
+        last < kBuckets - 1 && scale > 0.f ? (float)(last + 1) / scale * 1.000001f : INFINITY;
+    each_four(fmaxf(least_kept(), top - reach), [&](const float4& v, int i) {
       put(v.x, i);
       put(v.y, i + 1);
       put(v.z, i + 2);
       put(v.w, i + 3);
     });
     __syncthreads();
-    if (CL == 1) return true;
+    if (CL == 1) return s.fill;
     share(s.fills, s.fill);
-    if (rank != 0) return false;
-    if (tid < n) {
-      int r = 0, from = tid;
+    int n = 0;
 #pragma unroll
-      for (int q = 0; q < CL - 1; ++q)
-        if (r == q && from >= s.fills[q]) {
-          from -= s.fills[q];
-          ++r;
-        }
-      list()[tid] = of_rank(mine, r)[from];
+    for (int r = 0; r < CL; ++r) n += s.fills[r];
+    if (rank == 0 && n <= most) {
+      if (tid < n) {
+        int r = 0, from = tid;
+#pragma unroll
+        for (int q = 0; q < CL - 1; ++q)
+          if (r == q && from >= s.fills[q]) {
+            from -= s.fills[q];
+            ++r;
+          }
+        list()[tid] = of_rank(mine, r)[from];
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    return true;
+    return n;
   }
 
   // The list is not sorted: an entry's place in the falling order is what lies
@@ -443,8 +518,8 @@ struct Sampler {
 
   // CTA 0: the token among its list of n (the largest logits): at most the
   // first k (0: all), of these the shortest run that weighs `want` (0: the share
-  // P of their whole), min-p M, draw u.
-  __device__ void finish(int n, int k, u64 want, float P, float M, float u, int32_t* token) {
+  // P of their whole), min-p, draw u.
+  __device__ void finish(int n, int k, u64 want, float P, float u, int32_t* token) {
     const u64* entries = list();
     u64* w = weights();
     if (tid < n) w[tid] = fixed(of_order((uint32_t)(entries[tid] >> 32)));
@@ -466,7 +541,7 @@ struct Sampler {
       block_scan(keep && sh.q == 0 ? weight : 0, &total);
       want = P < 1.f ? want_of(P, total) : ~0ull;
     }
-    keep = keep && (ahead == 0 || mass < want) && !below(of_order((uint32_t)(me >> 32)), M);
+    keep = keep && (ahead == 0 || mass < want) && !below(of_order((uint32_t)(me >> 32)));
     block_scan(keep && sh.q == 0 ? weight : 0, &total);  // and every thread has read w
     if (mine && sh.q == 0 && !keep) w[sh.i] = 0;
     __syncthreads();
@@ -478,9 +553,8 @@ struct Sampler {
     if (keep && sh.q == 0 && lower <= point && lower + weight > point)
       *token = (int32_t)~(uint32_t)me;
   }
-  __device__ __forceinline__ bool below(float v, float M) const {  // exp((v - top) / T) < M
-    return M > 0.f && v != top &&
-           exp(((double)v - (double)top) * (c256 * (0.6931471805599453 / 256))) < (double)M;
+  __device__ __forceinline__ bool below(float v) const {  // exp((v - top) / T) < min-p
+    return (double)top - (double)v > reach_p;
   }
 
   // The cut in bucket `bkt`: among its logits gathered, or, for a bucket of
@@ -488,9 +562,9 @@ struct Sampler {
   // `need`: the amount still wanted of that bucket.
   template <bool MASS>
   __device__ void cut_in_bucket(int bkt, u64 need, int in_n) {
-    auto inside = [&](float v, int i) { return bucket(v) == bkt && kept(v, i); };
     if (in_n <= kList) {
-      if (gather(inside, in_n)) {
+      gather(bkt, bkt, kList);
+      if (rank == 0) {
         const u64* entries = list();
         u64* w = weights();
         if (tid < in_n) w[tid] = MASS ? fixed(of_order((uint32_t)(entries[tid] >> 32))) : 1;
@@ -515,8 +589,8 @@ struct Sampler {
     const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
     for (int d = 0; d < 3; ++d) {
       const uint32_t top_digit = (1u << bits[d]) - 1u;
-      const Border part = border<MASS>(
-          [&](float v, int i) { return inside(v, i) && (order_of(v) & mask) == prefix; },
+      const Border part = border<MASS, false>(
+          [&](float v) { return bucket(v) == bkt && (order_of(v) & mask) == prefix; },
           [&](float v) { return (int)(top_digit - ((order_of(v) >> shifts[d]) & top_digit)); },
           [&](u64) { return left; });
       prefix |= (top_digit - (uint32_t)part.bin) << shifts[d];
@@ -545,11 +619,33 @@ struct Sampler {
     cutting = true;
   }
 
-  // One filter: true when it ended the row (the token is written).
-  template <bool MASS, typename Want>
-  __device__ bool filter(Want want_of, int k, float P, float M, float u, int32_t* token) {
-    const Border edge = border<MASS>([&](float v, int i) { return kept(v, i); },
-                                   [&](float v) { return bucket(v); }, want_of);
+  // CTA 0 draws from what gather() listed; the others wait, their lists are read.
+  __device__ void finish_listed(int n, int k, u64 want, float P, float u,
+                                int32_t* token) {
+    if (rank == 0) finish(n, k, want, P, u, token);
+    sync();
+  }
+
+  // One filter, by count (the k largest) or by weight (the share P): true when
+  // it ended the row (the token is written).
+  template <bool MASS>
+  __device__ bool filter(int k, float P, float u, int32_t* token) {
+    auto any = [](float) { return true; };
+    auto bin = [&](float v) { return bucket(v); };
+    auto want = [&](u64 total) { return MASS ? want_of(P, total) : (u64)k; };
+    if (!MASS && k <= kFew) {
+      // The k-th largest of the batches' maxima is no larger than the k-th
+      // largest logit: what lies above it holds the k, and little more.
+      const Border edge = border<false, true>(any, bin, want);
+      if (edge.in_n > 0) {
+        const int n = gather(0, edge.bin, kFew);
+        if (n <= kFew) {
+          finish_listed(n, k, 0, P, u, token);
+          return true;
+        }
+      }
+    }
+    const Border edge = border<MASS, false>(any, bin, want);
     if (edge.in_n == 0) return false;  // fewer logits with a weight than k
     const int n = edge.above_n + edge.in_n;
     if (n > kFew) {
@@ -558,14 +654,13 @@ struct Sampler {
     }
     // After a histogram of weights the amount wanted is known, of the whole;
     // after one of counts, top-p is of the k that are left.
-    if (gather([&](float v, int i) { return bucket(v) <= edge.bin && kept(v, i); }, n))
-      finish(n, MASS ? 0 : k, MASS ? edge.want : 0, P, M, u, token);
-    sync();  // CTA 0 reads the others' lists
+    gather(0, edge.bin, kFew);
+    finish_listed(n, MASS ? 0 : k, MASS ? edge.want : 0, P, u, token);
     return true;
   }
 };
 
-template <int CL>
+template <int CL, bool RES>
 __global__ void __launch_bounds__(kThreads, 2)
     sample_kernel(const float* __restrict__ logits, int vocab, int slice, long long row_stride,
                   const float* __restrict__ uniforms, const float* __restrict__ temperature,
@@ -579,63 +674,51 @@ __global__ void __launch_bounds__(kThreads, 2)
   const float* src = logits + (size_t)row * row_stride + begin;
   // Logits before the first 16-byte boundary.
   const int head = min((int)((0u - (uint32_t)(reinterpret_cast<uintptr_t>(src) >> 2)) & 3u), len);
-  float* x = reinterpret_cast<float*>(smem + kScratchBytes);  // CL > 1
-
-  // The row's largest and least logit; with CL > 1 the CTA's logits also go into
-  // shared memory.
-  float hi = -INFINITY, lo = INFINITY;
-  int hi_at = 0;
-  auto see = [&](float v, int i) {
-    v = v != v ? -INFINITY : v + 0.f;  // -0 is +0
-    if (v > hi || (v == hi && begin + i < hi_at)) {
-      hi = v;
-      hi_at = begin + i;
-    }
-    if (v > -INFINITY) lo = fminf(lo, v);
-    return v;
-  };
   const int n4 = (len - head) / 4;
-  constexpr int kBatch = 8;
-  for (int base = tid; base < n4; base += kBatch * kThreads) {
-    float4 v[kBatch];
+  const int batches = (n4 + kQuads * kThreads - 1) / (kQuads * kThreads);
+  float* maxima = reinterpret_cast<float*>(smem + kScratchBytes);
+  // RES: the copy's quads lie on 16 bytes as the row's do.
+  float* x = maxima + batches_of(slice) * kThreads + ((4 - head) & 3);
+
+  // The row's largest and least logit, and every batch's largest; with RES the
+  // CTA's logits also go into shared memory.
+  float top = -INFINITY, lo = INFINITY;
+  auto canon = [](float v) { return Sampler<CL, RES>::canon(v); };
+  for (int it = 0; it < batches; ++it) {
+    const int base = it * kQuads * kThreads + tid;
+    float most = -INFINITY;
+    float4 v[kQuads];
 #pragma unroll
-    for (int e = 0; e < kBatch; ++e)
+    for (int e = 0; e < kQuads; ++e)
       if (base + e * kThreads < n4)
         v[e] = __ldg(reinterpret_cast<const float4*>(src + head) + base + e * kThreads);
 #pragma unroll
-    for (int e = 0; e < kBatch; ++e) {
-      const int i = head + 4 * (base + e * kThreads);
+    for (int e = 0; e < kQuads; ++e) {
       if (base + e * kThreads >= n4) break;
-      const float4 c = make_float4(see(v[e].x, i), see(v[e].y, i + 1), see(v[e].z, i + 2),
-                                   see(v[e].w, i + 3));
-      if (CL > 1) {
-        if (head == 0) {
-          *reinterpret_cast<float4*>(x + i) = c;
-        } else {
-          x[i] = c.x;
-          x[i + 1] = c.y;
-          x[i + 2] = c.z;
-          x[i + 3] = c.w;
-        }
-      }
+      const float4 c = make_float4(canon(v[e].x), canon(v[e].y), canon(v[e].z), canon(v[e].w));
+      most = max3(max3(most, c.x, c.y), c.z, c.w);
+      lo = fminf(lo, fminf(fminf(c.x, c.y), fminf(c.z, c.w)));
+      if (RES) *reinterpret_cast<float4*>(x + head + 4 * (base + e * kThreads)) = c;
     }
+    maxima[it * kThreads + tid] = most;
+    top = fmaxf(top, most);
   }
   const int tail = len - head - 4 * n4;
   if (tid < head + tail) {
     const int i = tid < head ? tid : len - tail + (tid - head);
-    const float c = see(src[i], i);
-    if (CL > 1) x[i] = c;
+    const float c = canon(src[i]);
+    top = fmaxf(top, c);
+    lo = fminf(lo, c);
+    if (RES) x[i] = c;
   }
-  u64 best = hi > -INFINITY ? ((u64)order_of(hi) << 32) | (uint32_t)~hi_at : 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const u64 c = __shfl_xor_sync(0xffffffffu, best, o);
-    best = c > best ? c : best;
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
   }
   if (lane == 0) {
-    s.warp[warp] = best;
-    s.warp_lo[warp] = lo;
+    s.warp_most[warp] = top;
+    s.warp_least[warp] = lo;
   }
   if (tid < 256) s.pow[tid] = g_powers.d[tid];
   float T = temperature ? temperature[row] : 1.f;
@@ -646,105 +729,181 @@ __global__ void __launch_bounds__(kThreads, 2)
   const float M = mp > 0.f ? fminf(mp, 1.f) : 0.f;
   const float u = uniforms[row];
   __syncthreads();
-  if (tid < CL) {
-    for (int w = 0; w < kWarps; ++w) {
-      best = s.warp[w] > best ? s.warp[w] : best;
-      lo = fminf(lo, s.warp_lo[w]);
+  for (int w = 0; w < kWarps; ++w) {
+    top = fmaxf(top, s.warp_most[w]);
+    lo = fminf(lo, s.warp_least[w]);
+  }
+  if (CL > 1) {
+    if (tid < CL) {
+      Sampler<CL, RES>::of_rank(s.most, tid)[rank] = top;
+      Sampler<CL, RES>::of_rank(s.least, tid)[rank] = lo;
     }
-    Sampler<CL>::of_rank(s.best, tid)[rank] = best;
-    Sampler<CL>::of_rank(s.least, tid)[rank] = lo;
-  }
-  Sampler<CL>::sync();
-  best = s.best[0];
-  lo = s.least[0];
+    Sampler<CL, RES>::sync();
 #pragma unroll
-  for (int r = 1; r < CL; ++r) {
-    best = s.best[r] > best ? s.best[r] : best;
-    lo = fminf(lo, s.least[r]);
+    for (int r = 0; r < CL; ++r) {
+      top = fmaxf(top, s.most[r]);
+      lo = fminf(lo, s.least[r]);
+    }
   }
-  if (best == 0 || !(T > 0.f)) {
-    if (rank == 0 && tid == 0) tokens[row] = best == 0 ? -1 : (int32_t)~(uint32_t)best;
+  if (top == -INFINITY) {
+    if (rank == 0 && tid == 0) tokens[row] = -1;
     return;
   }
-  float top = of_order((uint32_t)(best >> 32));
+  if (!(T > 0.f)) {  // the lowest index of the largest
+    int first = INT_MAX;
+    auto look = [&](float v, int i) {
+      if (canon(v) == top) first = min(first, begin + i);
+    };
+    const float* from = RES ? x : src;
+    for (int it = 0; it < batches; ++it)
+      if (maxima[it * kThreads + tid] == top)
+        for (int e = 0; e < kQuads; ++e) {
+          const int q = (it * kQuads + e) * kThreads + tid;
+          for (int j = 0; q < n4 && j < 4; ++j) look(from[head + 4 * q + j], head + 4 * q + j);
+        }
+    if (tid < head + tail) {
+      const int i = tid < head ? tid : len - tail + (tid - head);
+      look(from[i], i);
+    }
+    if (tid == 0) s.fill = INT_MAX;
+    __syncthreads();
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) atomicMin(&s.fill, first);
+    __syncthreads();
+    if (tid < CL) Sampler<CL, RES>::of_rank(s.where, tid)[rank] = s.fill;
+    Sampler<CL, RES>::sync();
+    if (rank == 0 && tid == 0) {
+      for (int r = 0; r < CL; ++r) first = min(first, s.where[r]);
+      tokens[row] = first;
+    }
+    return;
+  }
   const bool infinite = top == INFINITY;
   if (infinite) {  // these share the mass: zeros among -inf
-    if (CL > 1)
+    if (RES)
       for (int i = tid; i < len; i += kThreads) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
+    for (int it = 0; it < batches; ++it) {
+      float& most = maxima[it * kThreads + tid];
+      most = most == INFINITY ? 0.f : -INFINITY;
+    }
     __syncthreads();
     top = lo = 0.f;
   }
+  // A temperature below a 512th of the top's last place gives every other logit
+  // weight 0 as that 512th does, and keeps the distances' exponents in range.
+  const float under = nextafterf(top, -INFINITY);
+  T = fmaxf(T, (top - under) * (1.f / 512.f));
+  const float far = fmaxf(fminf(top - kFar * T, under), -FLT_MAX);
   // Buckets over the distances that have weight, or over the row's own range
-  // where that is narrower.
+  // where that is narrower (and not a masked row's, whose least is -inf).
   const float range = fminf(kFar * T, top - lo);
-  Sampler<CL> a = {s, CL > 1 ? x : src, smem, rank, begin, len, CL > 1 ? 0 : head, tid, lane, warp,
-                   top, fmaxf(top - kFar * T, -FLT_MAX), 369.3299304675746 / (double)T,
+  Sampler<CL, RES> a = {s, RES ? x : src, maxima, smem, rank, begin, len, head, tid, lane, warp,
+                   top, far, 369.3299304675746 / (double)T,
+               M > 0.f && T < INFINITY ? -log((double)M) * (double)T : (double)INFINITY,
                    range > 0.f ? (float)kBuckets / range : 0.f, infinite, false, {}};
-  if (k > 0 && k < vocab &&
-      a.template filter<false>([&](u64) { return (u64)k; }, k, P, M, u, tokens + row))
-    return;
-  if (P < 1.f &&
-      a.template filter<true>([&](u64 total) { return Sampler<CL>::want_of(P, total); }, k, P, M, u,
-                              tokens + row))
-    return;
-  // The draw by sums: warps take neighbouring segments of the CTA's quads, the
-  // first one also what comes before them, the last one what comes after.
-  // min-p: logits well above and below its distance need no exponential.
-  const float dist = T == INFINITY ? T : M > 0.f && M < 1.f ? (float)(-log((double)M) * T) : 0.f;
-  auto stays = [&](float v, int i) {
-    if (!a.kept(v, begin + i)) return false;
-    const float d = top - v;
-    return M == 0.f || d < dist * 0.99999f || (d <= dist * 1.00001f && !a.below(v, M));
-  };
+  if (k > 0 && k < vocab && a.template filter<false>(k, P, u, tokens + row)) return;
+  if (P < 1.f && a.template filter<true>(k, P, u, tokens + row)) return;
+  // The draw by sums, of every 128 neighbouring logits first.
+  auto stays = [&](float v, int i) { return a.kept(v, begin + i) && !a.below(v); };
+  // Nothing cut, and no weight at `far`: every logit goes into the sum as it is.
+  const bool simple = !a.cutting && M == 0.f && !infinite && a.far > -FLT_MAX;
   auto weight = [&](int i) -> u64 {
     const float v = a.at(i);
     return stays(v, i) ? a.fixed(v) : 0;
   };
-  const int all = a.n_quads(), part = (all + kWarps * 32 - 1) / (kWarps * 32) * 32;
-  u64 sum = 0;
-  a.quads(warp * part + lane, min((warp + 1) * part, all), 32, [&](const float4& v, int i) {
-    const bool k0 = stays(v.x, i), k1 = stays(v.y, i + 1), k2 = stays(v.z, i + 2),
-               k3 = stays(v.w, i + 3);
-    if (!(k0 || k1 || k2 || k3)) return;
-    const u64 f0 = a.fixed(v.x), f1 = a.fixed(v.y), f2 = a.fixed(v.z), f3 = a.fixed(v.w);
-    sum += ((k0 ? f0 : 0) + (k1 ? f1 : 0)) + ((k2 ? f2 : 0) + (k3 ? f3 : 0));
-  });
-  // Where segment w of the CTA starts.
-  auto start_of = [&](int w) {
-    return w == 0 ? 0 : w == kWarps ? len : a.head + 4 * min(w * part, all);
-  };
-  if (warp == 0 && lane < a.head) sum += weight(lane);
-  const int after = a.head + 4 * all;
-  if (warp == kWarps - 1 && lane < len - after) sum += weight(after + lane);
-  sum = warp_sum(sum);
+  // sums[0]: the logits before the quads; then one for each 32 quads; last: the
+  // logits after them.
+  u64* sums = reinterpret_cast<u64*>(smem);
+  const int parts = (a.n_quads() + 31) / 32 + 2;
+  // (min-p's distance with room for the roundings)
+  const float least = fmaxf(a.least_kept(), top - (float)a.reach_p * 1.00001f);
+  for (int it = 0; it < a.n_batches(); ++it) {
+    const bool active = maxima[it * kThreads + tid] >= least;  // -inf past the last quad
+    const int first = 1 + it * kQuads * kWarps + warp;
+    if (!__any_sync(0xffffffffu, active)) {
+      if (lane < kQuads && first + lane * kWarps < parts - 1) sums[first + lane * kWarps] = 0;
+      continue;
+    }
+#pragma unroll 1
+    for (int e0 = 0; e0 < kQuads; e0 += 4) {
+      float4 v[4];
+      double w[4];
+      if (simple) {
+        a.template half_batch<true>(it, e0, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = a.weigh4(v[e]);
+      } else {
+        a.half_batch(it, e0, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = a.place(it, e0 + e);
+          const bool k0 = stays(v[e].x, i), k1 = stays(v[e].y, i + 1), k2 = stays(v[e].z, i + 2),
+                     k3 = stays(v[e].w, i + 3);
+          w[e] = 0.0;
+          if (__any_sync(0xffffffffu, k0 || k1 || k2 || k3))
+            w[e] = ((k0 ? a.weigh(v[e].x) - kTwo52 : 0.0) + (k1 ? a.weigh(v[e].y) - kTwo52 : 0.0)) +
+                   ((k2 ? a.weigh(v[e].z) - kTwo52 : 0.0) + (k3 ? a.weigh(v[e].w) - kTwo52 : 0.0));
+        }
+      }
+      // The warp's four sums (of 128 weights, exact in FP64) at once: lanes of bit
+      // 4 take over two of them, lanes of bit 3 one of these; e is then (bit 4,
+      // bit 3).
+      const bool b4 = lane & 16, b3 = lane & 8;
+      const double x0 = (b4 ? w[2] : w[0]) + __shfl_xor_sync(0xffffffffu, b4 ? w[0] : w[2], 16);
+      const double x1 = (b4 ? w[3] : w[1]) + __shfl_xor_sync(0xffffffffu, b4 ? w[1] : w[3], 16);
+      double y = (b3 ? x1 : x0) + __shfl_xor_sync(0xffffffffu, b3 ? x0 : x1, 8);
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      const int to = first + (e0 + (lane >> 3)) * kWarps;
+      if ((lane & 7) == 0 && to < parts - 1) sums[to] = (u64)(long long)y;
+    }
+  }
+  if (tid < 2) {
+    u64 w = 0;
+    for (int i = tid ? a.head + 4 * a.n_quads() : 0; i < (tid ? len : a.head); ++i) w += weight(i);
+    sums[tid ? parts - 1 : 0] = w;
+  }
   __syncthreads();
-  if (lane == 0) s.warp[warp] = sum;
-  __syncthreads();
-  u64 mine = 0;
-  for (int w = 0; w < kWarps; ++w) mine += s.warp[w];
-  a.share(s.amount, mine);
+  const int each = (parts + kThreads - 1) / kThreads;
+  const int p0 = min(tid * each, parts), p1 = min(p0 + each, parts);
+  u64 mine = 0, all;
+  for (int p = p0; p < p1; ++p) mine += sums[p];
+  u64 run = a.block_scan(mine, &all);
+  a.share(s.amount, all);
   u64 total = 0, before = 0;
 #pragma unroll
   for (int r = 0; r < CL; ++r) {
     if (r < rank) before += s.amount[r];
     total += s.amount[r];
   }
-  const u64 point = Sampler<CL>::point_of(u, total);
-  if (before > point || before + mine <= point) return;
-  // The whole CTA goes over the segment that holds the point.
-  int seg = 0;
-  while (before + s.warp[seg] <= point) before += s.warp[seg++];
-  const int s0 = start_of(seg), s1 = start_of(seg + 1);
-  const int each = (s1 - s0 + kThreads - 1) / kThreads;
-  const int i0 = min(s0 + tid * each, s1), i1 = min(i0 + each, s1);
-  mine = 0;
-  for (int i = i0; i < i1; ++i) mine += weight(i);
-  u64 run = before + a.block_scan(mine, &total);
-  if (run > point || run + mine <= point) return;
-  for (int i = i0; i < i1; ++i) {
-    const u64 w = weight(i);
-    if (w && run <= point && run + w > point) tokens[row] = begin + i;
-    run += w;
+  const u64 point = Sampler<CL, RES>::point_of(u, total);
+  run += before;
+  if (run <= point && run + mine > point) {
+    int p = p0;
+    while (run + sums[p] <= point) run += sums[p++];
+    s.part = p;
+    s.run = run;
+  }
+  if (before > point || before + all <= point) return;
+  __syncthreads();
+  if (warp != 0) return;
+  // One warp goes over the 128 logits (or the few around the quads) at the point.
+  run = s.run;
+  const int at = s.part, end = a.head + 4 * a.n_quads();
+  const int i0 = at == 0 ? 0 : at == parts - 1 ? end : a.head + 128 * (at - 1);
+  const int i1 = at == 0 ? a.head : at == parts - 1 ? len : min(i0 + 128, end);
+  u64 w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int i = i0 + 4 * lane + e;
+    w[e] = i < i1 ? weight(i) : 0;
+  }
+  mine = (w[0] + w[1]) + (w[2] + w[3]);
+  run += warp_scan(mine, lane) - mine;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (w[e] && run <= point && run + w[e] > point) tokens[row] = begin + i0 + 4 * lane + e;
+    run += w[e];
   }
 }
 
@@ -755,19 +914,21 @@ using namespace tvp;
 
 namespace {
 
-template <int CL>
+template <int CL, bool RES>
 cudaError_t launch_sampler(int rows, int vocab, long long row_stride, const float* logits,
                            const float* uniforms, const float* temperature, const int32_t* top_k,
                            const float* top_p, const float* min_p, int32_t* tokens,
                            cudaStream_t stream) {
   auto slice_of = [](int v) { return CL > 1 ? ((v + CL - 1) / CL + 3) / 4 * 4 : v; };
-  auto smem_of = [](int slice) { return kScratchBytes + (CL > 1 ? (size_t)slice * 4 : 0); };
+  auto smem_of = [](int slice) {
+    return kScratchBytes + (size_t)batches_of(slice) * kThreads * 4 + (RES ? (size_t)slice * 4 + 16 : 0);
+  };
   static bool configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(sample_kernel<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(sample_kernel<CL, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)smem_of(slice_of(TVP_SAMPLE_MAX_VOCAB)));
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev] = true;
@@ -784,7 +945,7 @@ cudaError_t launch_sampler(int rows, int vocab, long long row_stride, const floa
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<CL>, logits, vocab, slice, row_stride, uniforms,
+  return cudaLaunchKernelEx(&cfg, sample_kernel<CL, RES>, logits, vocab, slice, row_stride, uniforms,
                             temperature, top_k, top_p, min_p, tokens);
 }
 
@@ -799,11 +960,10 @@ extern "C" int tvp_sample_tokens(const float* d_logits, int rows, int vocab, lon
     return TVP_ERR_INVALID_ARGUMENT;
   if (vocab > TVP_SAMPLE_MAX_VOCAB || rows > 65535) return TVP_ERR_UNSUPPORTED;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e =
-      rows < kStreamRows
-          ? launch_sampler<kCluster>(rows, vocab, row_stride, d_logits, d_uniforms, d_temperature,
-                                     d_top_k, d_top_p, d_min_p, d_tokens, st)
-          : launch_sampler<1>(rows, vocab, row_stride, d_logits, d_uniforms, d_temperature, d_top_k,
-                              d_top_p, d_min_p, d_tokens, st);
+  const auto launch = rows < kStreamRows   ? launch_sampler<kCluster, true>
+                      : rows < kStreamMany ? launch_sampler<4, false>
+                                           : launch_sampler<2, false>;
+  const cudaError_t e = launch(rows, vocab, row_stride, d_logits, d_uniforms, d_temperature,
+                               d_top_k, d_top_p, d_min_p, d_tokens, st);
   return e == cudaSuccess ? TVP_OK : TVP_ERR_RUNTIME;
 }
