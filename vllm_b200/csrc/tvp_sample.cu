@@ -45,9 +45,9 @@ static_assert(kBlocks == 64 && kBuckets / kCluster % 32 == 0, "border() deals th
 // Few rows: 8 CTAs keep a row in shared memory.  From kStreamRows on, 4 CTAs per
 // row read it again from L2 (kStreamMany: 2), which leaves room for more rows at
 // once.  Measured, us for rows of 128256 of mixed settings, 8 kept / 4 / 2
-// streaming: 32 rows 32 / 49 / 84, 64 rows 50 / 55 / 85, 96 rows 69 / 64 / 79,
-// 256 rows 157 / 127 / 127, 512 rows 294 / 218 / 194; of top-k 50: 32 rows
-// 14 / 14 / 17, 64 rows 26 / 17 / 17, 256 rows 102 / 67 / 49.
+// streaming: 32 rows 32 / 46 / 76, 64 rows 50 / 51 / 77, 96 rows 69 / 60 / 71,
+// 256 rows 157 / 115 / 117; of top-k 50: 32 rows 14 / 14 / 17, 64 rows
+// 27 / 16 / 17, 256 rows 105 / 65 / 47.
 constexpr int kStreamRows = 64;
 constexpr int kStreamMany = 192;
 constexpr int kList = 512;  // logits of a bucket that CTA 0 takes in
@@ -61,14 +61,14 @@ constexpr float kFar = 33.f;
 constexpr double kTwo52 = 4503599627370496.0;
 
 struct Cut {
-  uint32_t key;  // kept: order image above it, or equal and index <= last
+  float value;  // kept: logits above it, or equal and of index <= last
   int last;
 };
 
-// The bin where a running amount reaches `want`: the amount before it, and the
-// counts before and in it (0: the amount is not reached).
+// The bin where a running amount reaches `want`, and the amount before it; bin
+// kBuckets: it is not reached.
 struct Border {
-  int bin, above_n, in_n;
+  int bin;
   u64 above, want;
 };
 
@@ -78,12 +78,10 @@ struct alignas(16) Shared {
   float most[CL], least[CL];  // by rank: largest and least logit
   int where[CL];              // by rank: the lowest index of the largest
   u64 amount[CL];  // by rank: a sum that the step at hand exchanges
-  int fills[CL];
+  int fills[2][CL];  // in turn: one gather() may follow another at once
   u64 ties[CL];
-  u64 seg[CL > 1 ? kSegment : 1];         // this CTA's segment of the cluster's histogram: amounts
-  uint32_t seg_n[CL > 1 ? kSegment : 1];  // and counts
-  u64 sub[kBlocks];                       // every 32 buckets of the whole histogram: amounts
-  uint32_t sub_n[kBlocks];                // and counts
+  u64 seg[CL > 1 ? kSegment : 1];  // this CTA's segment of the cluster's histogram
+  u64 sub[kBlocks];                // every 32 buckets of the whole histogram
   u64 warp[kWarps];
   float warp_most[kWarps], warp_least[kWarps];
   double pow[256];
@@ -111,7 +109,7 @@ struct Powers {
 };
 __device__ const Powers g_powers = Powers();
 
-constexpr size_t kScratchBytes = kBuckets * 12;  // histogram, then the lists
+constexpr size_t kScratchBytes = kBuckets * 8 + 5120;  // histogram, then the lists
 static_assert(kScratchBytes >= 3 * kList * 8, "the lists fit the histogram's place");
 static_assert(kScratchBytes >= (TVP_SAMPLE_MAX_VOCAB / 128 + 3) * 8, "and so do the sums");
 
@@ -120,7 +118,7 @@ __host__ __device__ constexpr int batches_of(int logits) {
 }
 
 __device__ __forceinline__ uint32_t order_of(float x) {  // larger logit, larger image
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.f);  // -0 is +0
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float of_order(uint32_t o) {
@@ -140,6 +138,20 @@ __device__ __forceinline__ V warp_scan(V v, int lane) {  // inclusive
     if (lane >= o) v += y;
   }
   return v;
+}
+
+// Exclusive sum over the block's threads (all must call), and the total; `sums`:
+// shared memory, one per warp.
+__device__ u64 block_scan(u64* sums, u64 v, u64* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const u64 inc = warp_scan(v, lane);
+  __syncthreads();
+  if (lane == 31) sums[warp] = inc;
+  __syncthreads();
+  const u64 w = lane < kWarps ? sums[lane] : 0;
+  const u64 winc = warp_scan(w, lane);
+  *total = __shfl_sync(0xffffffffu, winc, 31);
+  return __shfl_sync(0xffffffffu, winc - w, warp) + inc - v;
 }
 
 // 64-bit sum into shared memory from two 32-bit ones: the low words' carry goes
@@ -165,9 +177,9 @@ struct Sampler {
   double c256;  // 256 log2(e) / T
   double reach_p;  // min-p keeps the logits up to this far below the top
   float scale;  // buckets per unit of distance
-  bool infinite;  // the row holds +inf: these count as 0, the others as -inf
-  bool cutting;  // a filter has cut the row
-  Cut cut;
+  float least;  // what the filters have left of the row: see kept()
+  int last;
+  int turn;
 
   // The CTAs of a row: barrier, and another one's shared memory.
   __device__ static void sync() {
@@ -181,24 +193,13 @@ struct Sampler {
     return CL > 1 ? cg::this_cluster().map_shared_rank(place, r) : place;
   }
 
-  // A logit as the sampler takes it: NaN is -inf, -0 is +0; in a row with +inf
-  // these count as 0, the others as -inf.  Shared memory holds them so.
-  __device__ __forceinline__ static float canon(float v) { return fmaxf(v + 0.f, -INFINITY); }
-  __device__ __forceinline__ static float only(float v) { return v == INFINITY ? 0.f : -INFINITY; }
-  __device__ __forceinline__ float at(int i) const {
-    if (RES) return x[i];
-    return infinite ? only(x[i]) : canon(x[i]);
-  }
-
   // A thread's batch `it` is the kQuads quads of logits (it kQuads + e) kThreads +
   // tid after the head: a warp's quads of one e are 128 neighbouring logits.
   __device__ __forceinline__ int n_quads() const { return (len - head) / 4; }
   __device__ __forceinline__ int n_batches() const {
     return (n_quads() + kQuads * kThreads - 1) / (kQuads * kThreads);
   }
-  // Quads e0 .. e0 + 3 of batch `it`, -inf past the last one, as they are stored
-  // or as the sampler takes them.
-  template <bool RAW = false>
+  // Quads e0 .. e0 + 3 of batch `it`, -inf past the last one.
   __device__ __forceinline__ void half_batch(int it, int e0, float4 (&v)[4]) const {
     const float4* x4 = reinterpret_cast<const float4*>(x + head);
     const int n4 = n_quads();
@@ -207,51 +208,37 @@ struct Sampler {
       const int q = (it * kQuads + e0 + e) * kThreads + tid;
       v[e] = q < n4 ? x4[q] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     }
-    if (RES || RAW) return;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      v[e] = make_float4(canon(v[e].x), canon(v[e].y), canon(v[e].z), canon(v[e].w));
-    if (infinite) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        v[e] = make_float4(only(v[e].x), only(v[e].y), only(v[e].z), only(v[e].w));
-    }
   }
   // Index of the first logit of quad e of batch `it`.
   __device__ __forceinline__ int place(int it, int e) const {
     return head + 4 * ((it * kQuads + e) * kThreads + tid);
   }
   // Calls visit(four logits, index of the first) for the CTA's logits; batches
-  // whose largest is below `least` are left out.  The logits around the quads
+  // whose largest is below `floor` are left out.  The logits around the quads
   // come as fours with -inf.
   template <typename Visit>
-  __device__ __forceinline__ void each_four(float least, Visit visit) const {
+  __device__ __forceinline__ void each_four(float floor, Visit visit) const {
     const int n = n_batches();
     for (int it = 0; it < n; ++it) {
-      if (maxima[it * kThreads + tid] < least) continue;
+      if (maxima[it * kThreads + tid] < floor) continue;
 #pragma unroll 1  // the code of a pass is fetched once per row: it had better be short
       for (int e0 = 0; e0 < kQuads; e0 += 4) {
         float4 v[4];
         half_batch(it, e0, v);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (fmaxf(fmaxf(v[e].x, v[e].y), fmaxf(v[e].z, v[e].w)) >= least)
+          if (fmaxf(fmaxf(v[e].x, v[e].y), fmaxf(v[e].z, v[e].w)) >= floor)
             visit(v[e], place(it, e0 + e));
       }
     }
     const int i = single();
-    if (i >= 0) visit(make_float4(at(i), -INFINITY, -INFINITY, -INFINITY), i);
+    if (i >= 0) visit(make_float4(x[i], -INFINITY, -INFINITY, -INFINITY), i);
   }
   // This thread's logit among the up to 6 before and after the quads, or -1.
   __device__ __forceinline__ int single() const {
     const int tail = (len - head) & 3;
     return tid < head ? tid : tid < head + tail ? len - tail + (tid - head) : -1;
   }
-  // No kept logit is below this.
-  __device__ __forceinline__ float least_kept() const {
-    return cutting ? fmaxf(far, of_order(cut.key)) : far;
-  }
-
   // 2^52 + the weight of a logit in 2^-44 of the largest's: the sum's mantissa
   // holds the integer.  Without branches, so that the chains of several logits
   // overlap; a logit below `far`, a NaN among them, counts as `far`, which rounds
@@ -282,24 +269,13 @@ struct Sampler {
   __device__ __forceinline__ int bucket(float v) const {  // rises as v falls
     return (int)fminf((top - v) * scale, (float)(kBuckets - 1));
   }
-  __device__ __forceinline__ bool kept(float v, int i) const {  // with a weight, that is
-    if (v < far) return false;
-    if (!cutting) return true;
-    const uint32_t o = order_of(v);
-    return o > cut.key || (o == cut.key && i <= cut.last);
+  // No kept logit is below `least`; of those equal to it the ones up to `last`.  A
+  // NaN is not kept.
+  __device__ __forceinline__ bool kept(float v, int i) const {
+    return v > least || (v == least && i <= last);
   }
-  // Exclusive sum over the block's threads (all must call), and the total.
-  __device__ u64 block_scan(u64 v, u64* total) {
-    const u64 inc = warp_scan(v, lane);
-    __syncthreads();
-    if (lane == 31) s.warp[warp] = inc;
-    __syncthreads();
-    const u64 w = lane < kWarps ? s.warp[lane] : 0;
-    const u64 winc = warp_scan(w, lane);
-    *total = __shfl_sync(0xffffffffu, winc, 31);
-    const u64 before = __shfl_sync(0xffffffffu, winc - w, warp);
-    return before + inc - v;
-  }
+
+  __device__ u64 block_scan(u64 v, u64* total) { return tvp::block_scan(s.warp, v, total); }
 
   // Every CTA's value, to every CTA's `place[rank]`; a cluster barrier inside.
   // Between two calls with one place every CTA passes another cluster barrier
@@ -318,26 +294,27 @@ struct Sampler {
   template <bool MASS, bool MAXIMA, typename Take, typename Bin, typename Want>
   __device__ Border border(Take take, Bin bin, Want want_of) {
     u64* hist = reinterpret_cast<u64*>(scratch);
-    uint32_t* hist_n = reinterpret_cast<uint32_t*>(hist + kBuckets);
-    for (int i = tid; i < (int)(kScratchBytes / 16); i += kThreads)
+    uint32_t* counts = reinterpret_cast<uint32_t*>(scratch);
+    for (int i = tid; i < kBuckets * (MASS ? 8 : 4) / 16; i += kThreads)
       reinterpret_cast<uint4*>(scratch)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     auto add = [&](float v, u64 w, int i) {
       if (!kept(v, begin + i) || !take(v)) return;
-      const int b = bin(v);
-      atomicAdd(&hist_n[b], 1u);
-      if (MASS) shared_add(&hist[b], w);
+      if (MASS)
+        shared_add(&hist[bin(v)], w);
+      else
+        atomicAdd(&counts[bin(v)], 1u);
     };
     if (MAXIMA) {
       const int n = n_batches();
       for (int it = 0; it < n; ++it) {
         const float v = maxima[it * kThreads + tid];
-        if (v >= far) atomicAdd(&hist_n[bin(v)], 1u);
+        if (v >= far) atomicAdd(&counts[bin(v)], 1u);
       }
       const int i = single();
-      if (i >= 0) add(at(i), 0, i);
+      if (i >= 0) add(x[i], 0, i);
     } else {
-      each_four(least_kept(), [&](const float4& v, int i) {
+      each_four(least, [&](const float4& v, int i) {
         u64 w[4] = {};
         if (MASS) {
           w[0] = fixed(v.x);
@@ -357,37 +334,20 @@ struct Sampler {
       // every CTA.
       for (int i = tid; i < kSegment; i += kThreads) {
         const int b = rank * kSegment + i;
-        uint32_t ns[CL];
-        u64 as[CL];
+        u64 as[CL], a = 0;
 #pragma unroll
-        for (int r = 0; r < CL; ++r) {
-          ns[r] = of_rank(hist_n, r)[b];
-          if (MASS) as[r] = of_rank(hist, r)[b];
-        }
-        uint32_t n = 0;
-        u64 a = 0;
+        for (int r = 0; r < CL; ++r) as[r] = MASS ? of_rank(hist, r)[b] : of_rank(counts, r)[b];
 #pragma unroll
-        for (int r = 0; r < CL; ++r) {
-          n += ns[r];
-          a += MASS ? as[r] : ns[r];
-        }
+        for (int r = 0; r < CL; ++r) a += as[r];
         s.seg[i] = a;
-        s.seg_n[i] = n;
-        a = MASS ? warp_sum(a) : 0;
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (lane < CL) {
-          of_rank(s.sub, lane)[b / 32] = MASS ? a : n;
-          of_rank(s.sub_n, lane)[b / 32] = n;
-        }
+        a = warp_sum(a);
+        if (lane < CL) of_rank(s.sub, lane)[b / 32] = a;
       }
     } else {
       for (int block = warp; block < kBlocks; block += kWarps) {
-        const uint32_t n = __reduce_add_sync(0xffffffffu, hist_n[block * 32 + lane]);
-        const u64 a = MASS ? warp_sum(hist[block * 32 + lane]) : n;
-        if (lane == 0) {
-          s.sub[block] = a;
-          s.sub_n[block] = n;
-        }
+        const int i = block * 32 + lane;
+        const u64 a = warp_sum(MASS ? hist[i] : counts[i]);
+        if (lane == 0) s.sub[block] = a;
       }
     }
     sync();
@@ -400,17 +360,13 @@ struct Sampler {
   __device__ __forceinline__ void find_border(Want want_of) {
     Border out;
     const u64 s0 = s.sub[2 * lane], s1 = s.sub[2 * lane + 1];
-    const uint32_t n0 = s.sub_n[2 * lane], n1 = s.sub_n[2 * lane + 1];
     const u64 inc = warp_scan(s0 + s1, lane);
-    const uint32_t inc_n = warp_scan(n0 + n1, lane);
     out.want = want_of(__shfl_sync(0xffffffffu, inc, 31));
     const u64 before = inc - s0 - s1;
     const uint32_t at = __ballot_sync(0xffffffffu, before < out.want && inc >= out.want);
     if (at == 0) {
-      out.bin = kBuckets - 1;
-      out.above = __shfl_sync(0xffffffffu, inc, 31);
-      out.above_n = (int)__shfl_sync(0xffffffffu, inc_n, 31);
-      out.in_n = 0;
+      out.bin = kBuckets;
+      out.above = 0;
       if (lane == 0) s.border = out;
       return;
     }
@@ -418,49 +374,55 @@ struct Sampler {
     const bool second = before + s0 < out.want;
     const int block = 2 * src + __shfl_sync(0xffffffffu, (int)second, src);
     const u64 above = __shfl_sync(0xffffffffu, second ? before + s0 : before, src);
-    const uint32_t above_n =
-        __shfl_sync(0xffffffffu, second ? inc_n - n1 : inc_n - n0 - n1, src);
-    u64 ba;
-    uint32_t bn;
+    u64 mine;
     if (CL > 1) {
       constexpr int kPer = kSegment / 32;  // blocks of a CTA
-      const int place = block % kPer * 32 + lane;
-      ba = of_rank(s.seg, block / kPer)[place];
-      bn = of_rank(s.seg_n, block / kPer)[place];
+      mine = of_rank(s.seg, block / kPer)[block % kPer * 32 + lane];
     } else {
-      const u64* hist = reinterpret_cast<const u64*>(scratch);
-      bn = reinterpret_cast<const uint32_t*>(hist + kBuckets)[block * 32 + lane];
-      ba = MASS ? hist[block * 32 + lane] : bn;
+      mine = MASS ? reinterpret_cast<const u64*>(scratch)[block * 32 + lane]
+                  : reinterpret_cast<const uint32_t*>(scratch)[block * 32 + lane];
     }
-    const u64 upto = above + warp_scan(ba, lane);
-    const uint32_t upto_n = above_n + warp_scan(bn, lane);
+    const u64 upto = above + warp_scan(mine, lane);
     const int hit = __ffs(__ballot_sync(0xffffffffu, upto >= out.want)) - 1;
     out.bin = block * 32 + hit;
-    out.above = __shfl_sync(0xffffffffu, upto - ba, hit);
-    out.above_n = (int)__shfl_sync(0xffffffffu, upto_n - bn, hit);
-    out.in_n = (int)__shfl_sync(0xffffffffu, bn, hit);
+    out.above = __shfl_sync(0xffffffffu, upto - mine, hit);
     if (lane == 0) s.border = out;
   }
 
-  // The kept logits in buckets first .. last, as (order image, ~index), in CTA
-  // 0's list, in no order; returns how many there are in the row.  More than
-  // `most` (<= kList) are not listed.
+  // The kept logits in buckets b0 .. b1, as (order image, ~index), in CTA
+  // 0's list, in no order; returns how many there are in the row, or, when more
+  // than `most` (<= kList), some number above that and no list.
   __device__ u64* list() const { return reinterpret_cast<u64*>(scratch) + kList; }
   __device__ u64* weights() const { return reinterpret_cast<u64*>(scratch) + 2 * kList; }
-  __device__ int gather(int first, int last, int most) {
+  __device__ int gather(int b0, int b1, int most) {
     u64* mine = CL == 1 ? list() : reinterpret_cast<u64*>(scratch);
+    // A logit of bucket b1 lies above this (the distance is rounded, by 2^-23 of it
+    // at most, and so are the product and the quotient).
+    const float reach =
+        b1 < kBuckets - 1 && scale > 0.f ? (float)(b1 + 1) / scale * 1.000001f : INFINITY;
+    const float floor = fmaxf(least, top - reach);
     if (tid == 0) s.fill = 0;
     __syncthreads();
+    if (b0 == 0) {  // at least one logit for each batch whose largest lies there
+      int n = 0;
+      for (int it = 0; it < n_batches(); ++it) n += bucket(maxima[it * kThreads + tid]) <= b1 &&
+                                                    maxima[it * kThreads + tid] > least;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane == 0 && n > 0) atomicAdd(&s.fill, n);
+      __syncthreads();
+      n = s.fill;
+      __syncthreads();
+      if (n <= most && tid == 0) s.fill = 0;
+      __syncthreads();
+    }
     auto put = [&](float v, int i) {
-      if (!kept(v, begin + i) || bucket(v) < first || bucket(v) > last) return;
+      if (!kept(v, begin + i) || bucket(v) < b0 || bucket(v) > b1) return;
+      // past `most` the count no longer matters
+      if (*const_cast<volatile int*>(&s.fill) > most) return;
       const int to = atomicAdd(&s.fill, 1);
       if (to < most) mine[to] = ((u64)order_of(v) << 32) | (uint32_t)~(begin + i);
     };
-    // A logit of bucket `last` lies above this (the distance is rounded, by 2^-23
-    // of it at most, and so are the product and the quotient).
-    const float reach =
-        last < kBuckets - 1 && scale > 0.f ? (float)(last + 1) / scale * 1.000001f : INFINITY;
-    each_four(fmaxf(least_kept(), top - reach), [&](const float4& v, int i) {
+    if (*const_cast<volatile int*>(&s.fill) <= most) each_four(floor, [&](const float4& v, int i) {
       put(v.x, i);
       put(v.y, i + 1);
       put(v.z, i + 2);
@@ -468,17 +430,18 @@ struct Sampler {
     });
     __syncthreads();
     if (CL == 1) return s.fill;
-    share(s.fills, s.fill);
+    int* fills = s.fills[turn ^= 1];
+    share(fills, s.fill);
     int n = 0;
 #pragma unroll
-    for (int r = 0; r < CL; ++r) n += s.fills[r];
+    for (int r = 0; r < CL; ++r) n += fills[r];
     if (rank == 0 && n <= most) {
       if (tid < n) {
         int r = 0, from = tid;
 #pragma unroll
         for (int q = 0; q < CL - 1; ++q)
-          if (r == q && from >= s.fills[q]) {
-            from -= s.fills[q];
+          if (r == q && from >= fills[q]) {
+            from -= fills[q];
             ++r;
           }
         list()[tid] = of_rank(mine, r)[from];
@@ -561,9 +524,9 @@ struct Sampler {
   // many, by radix digits of the order image and, among equal logits, by index.
   // `need`: the amount still wanted of that bucket.
   template <bool MASS>
-  __device__ void cut_in_bucket(int bkt, u64 need, int in_n) {
+  __device__ void cut_in_bucket(int bkt, u64 need) {
+    const int in_n = gather(bkt, bkt, kList);
     if (in_n <= kList) {
-      gather(bkt, bkt, kList);
       if (rank == 0) {
         const u64* entries = list();
         u64* w = weights();
@@ -575,13 +538,13 @@ struct Sampler {
         for (int j = sh.q; j < in_n; j += sh.parts) ahead += entries[j] > me ? w[j] : 0;
         ahead = over_parts(ahead, sh.parts);
         if (sh.i < in_n && sh.q == 0 && ahead < need && ahead + w[sh.i] >= need) {
-          const Cut c = {(uint32_t)(me >> 32), (int)~(uint32_t)me};
+          const Cut c = {of_order((uint32_t)(me >> 32)), (int)~(uint32_t)me};
           for (int r = 0; r < CL; ++r) *of_rank(&s.cut, r) = c;
         }
       }
       sync();
-      cut = s.cut;
-      cutting = true;
+      least = s.cut.value;
+      last = s.cut.last;
       return;
     }
     uint32_t prefix = 0, mask = 0;
@@ -603,20 +566,20 @@ struct Sampler {
     const int each = (len + kThreads - 1) / kThreads;
     const int i0 = min(tid * each, len), i1 = min(i0 + each, len);
     u64 ties = 0, all;
-    for (int i = i0; i < i1; ++i) ties += kept(at(i), begin + i) && order_of(at(i)) == prefix;
+    for (int i = i0; i < i1; ++i) ties += kept(x[i], begin + i) && order_of(x[i]) == prefix;
     const u64 before = block_scan(ties, &all);
     share(s.ties, all);
     u64 seen = before;
     for (int r = 0; r < rank; ++r) seen += s.ties[r];
-    int last = -1;
+    int nth_at = -1;
     if (seen < nth && seen + ties >= nth)
       for (int i = i0; i < i1; ++i)
-        if (kept(at(i), begin + i) && order_of(at(i)) == prefix && ++seen == nth) last = begin + i;
-    if (last >= 0)
-      for (int r = 0; r < CL; ++r) *of_rank(&s.cut, r) = {prefix, last};
+        if (kept(x[i], begin + i) && order_of(x[i]) == prefix && ++seen == nth) nth_at = begin + i;
+    if (nth_at >= 0)
+      for (int r = 0; r < CL; ++r) *of_rank(&s.cut, r) = {of_order(prefix), nth_at};
     sync();
-    cut = s.cut;
-    cutting = true;
+    least = s.cut.value;
+    last = s.cut.last;
   }
 
   // CTA 0 draws from what gather() listed; the others wait, their lists are read.
@@ -637,7 +600,7 @@ struct Sampler {
       // The k-th largest of the batches' maxima is no larger than the k-th
       // largest logit: what lies above it holds the k, and little more.
       const Border edge = border<false, true>(any, bin, want);
-      if (edge.in_n > 0) {
+      if (edge.bin < kBuckets) {
         const int n = gather(0, edge.bin, kFew);
         if (n <= kFew) {
           finish_listed(n, k, 0, P, u, token);
@@ -646,17 +609,18 @@ struct Sampler {
       }
     }
     const Border edge = border<MASS, false>(any, bin, want);
-    if (edge.in_n == 0) return false;  // fewer logits with a weight than k
-    const int n = edge.above_n + edge.in_n;
-    if (n > kFew) {
-      cut_in_bucket<MASS>(edge.bin, edge.want - edge.above, edge.in_n);
-      return false;
+    if (edge.bin == kBuckets) return false;  // fewer logits with a weight than k
+    if (MASS || k <= kFew) {
+      // After a histogram of weights the amount wanted is known, of the whole;
+      // after one of counts, top-p is of the k that are left.
+      const int n = gather(0, edge.bin, kFew);
+      if (n <= kFew) {
+        finish_listed(n, MASS ? 0 : k, MASS ? edge.want : 0, P, u, token);
+        return true;
+      }
     }
-    // After a histogram of weights the amount wanted is known, of the whole;
-    // after one of counts, top-p is of the k that are left.
-    gather(0, edge.bin, kFew);
-    finish_listed(n, MASS ? 0 : k, MASS ? edge.want : 0, P, u, token);
-    return true;
+    cut_in_bucket<MASS>(edge.bin, edge.want - edge.above);
+    return false;
   }
 };
 
@@ -683,7 +647,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   // The row's largest and least logit, and every batch's largest; with RES the
   // CTA's logits also go into shared memory.
   float top = -INFINITY, lo = INFINITY;
-  auto canon = [](float v) { return Sampler<CL, RES>::canon(v); };
   for (int it = 0; it < batches; ++it) {
     const int base = it * kQuads * kThreads + tid;
     float most = -INFINITY;
@@ -695,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
     for (int e = 0; e < kQuads; ++e) {
       if (base + e * kThreads >= n4) break;
-      const float4 c = make_float4(canon(v[e].x), canon(v[e].y), canon(v[e].z), canon(v[e].w));
+      const float4 c = v[e];  // a NaN loses every comparison
       most = max3(max3(most, c.x, c.y), c.z, c.w);
       lo = fminf(lo, fminf(fminf(c.x, c.y), fminf(c.z, c.w)));
       if (RES) *reinterpret_cast<float4*>(x + head + 4 * (base + e * kThreads)) = c;
@@ -706,7 +669,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int tail = len - head - 4 * n4;
   if (tid < head + tail) {
     const int i = tid < head ? tid : len - tail + (tid - head);
-    const float c = canon(src[i]);
+    const float c = src[i];
     top = fmaxf(top, c);
     lo = fminf(lo, c);
     if (RES) x[i] = c;
@@ -752,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (!(T > 0.f)) {  // the lowest index of the largest
     int first = INT_MAX;
     auto look = [&](float v, int i) {
-      if (canon(v) == top) first = min(first, begin + i);
+      if (v == top) first = min(first, begin + i);
     };
     const float* from = RES ? x : src;
     for (int it = 0; it < batches; ++it)
@@ -778,16 +741,28 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     return;
   }
-  const bool infinite = top == INFINITY;
-  if (infinite) {  // these share the mass: zeros among -inf
-    if (RES)
-      for (int i = tid; i < len; i += kThreads) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
-    for (int it = 0; it < batches; ++it) {
-      float& most = maxima[it * kThreads + tid];
-      most = most == INFINITY ? 0.f : -INFINITY;
+  if (top == INFINITY) {
+    // These alone have weight, the same each: the filters leave the first n of
+    // them, and the draw takes one of these by its place.
+    const int each = (len + kThreads - 1) / kThreads;
+    const int i0 = min(tid * each, len), i1 = min(i0 + each, len);
+    const float* from = RES ? x : src;
+    u64 count = 0, all;
+    for (int i = i0; i < i1; ++i) count += from[i] == INFINITY;
+    u64 seen = block_scan(s.warp, count, &all);
+    if (tid < CL) Sampler<CL, RES>::of_rank(s.amount, tid)[rank] = all;
+    Sampler<CL, RES>::sync();
+    u64 n = 0;
+    for (int r = 0; r < CL; ++r) {
+      if (r < rank) seen += s.amount[r];
+      n += s.amount[r];
     }
-    __syncthreads();
-    top = lo = 0.f;
+    if (k > 0) n = min(n, (u64)k);
+    if (P < 1.f) n = Sampler<CL, RES>::want_of(P, n);
+    const u64 place = Sampler<CL, RES>::point_of(u, n);
+    for (int i = i0; i < i1; ++i)
+      if (from[i] == INFINITY && seen++ == place) tokens[row] = begin + i;
+    return;
   }
   // A temperature below a 512th of the top's last place gives every other logit
   // weight 0 as that 512th does, and keeps the distances' exponents in range.
@@ -800,15 +775,17 @@ __global__ void __launch_bounds__(kThreads, 2)
   Sampler<CL, RES> a = {s, RES ? x : src, maxima, smem, rank, begin, len, head, tid, lane, warp,
                    top, far, 369.3299304675746 / (double)T,
                M > 0.f && T < INFINITY ? -log((double)M) * (double)T : (double)INFINITY,
-                   range > 0.f ? (float)kBuckets / range : 0.f, infinite, false, {}};
+                   range > 0.f ? (float)kBuckets / range : 0.f, far, INT_MAX, 0};
   if (k > 0 && k < vocab && a.template filter<false>(k, P, u, tokens + row)) return;
   if (P < 1.f && a.template filter<true>(k, P, u, tokens + row)) return;
   // The draw by sums, of every 128 neighbouring logits first.
-  auto stays = [&](float v, int i) { return a.kept(v, begin + i) && !a.below(v); };
+  auto stays = [&](float v, int i) {
+    return a.kept(v, begin + i) && (M == 0.f || !a.below(v));
+  };
   // Nothing cut, and no weight at `far`: every logit goes into the sum as it is.
-  const bool simple = !a.cutting && M == 0.f && !infinite && a.far > -FLT_MAX;
+  const bool simple = a.least == far && M == 0.f && far > -FLT_MAX;
   auto weight = [&](int i) -> u64 {
-    const float v = a.at(i);
+    const float v = a.x[i];
     return stays(v, i) ? a.fixed(v) : 0;
   };
   // sums[0]: the logits before the quads; then one for each 32 quads; last: the
@@ -816,7 +793,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   u64* sums = reinterpret_cast<u64*>(smem);
   const int parts = (a.n_quads() + 31) / 32 + 2;
   // (min-p's distance with room for the roundings)
-  const float least = fmaxf(a.least_kept(), top - (float)a.reach_p * 1.00001f);
+  const float least = fmaxf(a.least, top - (float)a.reach_p * 1.00001f);
   for (int it = 0; it < a.n_batches(); ++it) {
     const bool active = maxima[it * kThreads + tid] >= least;  // -inf past the last quad
     const int first = 1 + it * kQuads * kWarps + warp;
@@ -829,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       float4 v[4];
       double w[4];
       if (simple) {
-        a.template half_batch<true>(it, e0, v);
+        a.half_batch(it, e0, v);
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = a.weigh4(v[e]);
       } else {
