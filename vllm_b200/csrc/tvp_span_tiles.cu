@@ -288,7 +288,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (lane == 0) {
       constexpr uint32_t kIdS = umma_idesc_bf16_f32(kRows, kChunk, false, false);
       constexpr uint32_t kIdO = umma_idesc_bf16_f32(kRows, kHeadDim, false, true);
-      auto stage_k = [&](int c) { return sbase + kOffStages + (c % kStages) * kChunkBytes; };
+      // Descriptors of Q and of stage 0's K and V; a byte offset adds offset / 16.
+      const uint64_t q_desc = umma_desc_sw128(sbase, 16, 1024);
+      const uint64_t k_desc = umma_desc_sw128(sbase + kOffStages, 16, 1024);
+      const uint64_t v_desc = umma_desc_sw128(sbase + kOffStages + kKvBytes, 0, 1024);
       bool ok = true;
       auto wait = [&](uint32_t b, uint32_t parity) {
         if (ok && !mbar_wait_bounded(b, parity)) {
@@ -298,30 +301,36 @@ __global__ void __launch_bounds__(kThreads, 2)
         return ok;
       };
       // S(c) = Q K(c)^T into the columns of side c % 2, 16 channels per MMA.
+      int s_stage = 0, s_parity = 0;  // of the next chunk of S
       auto issue_s = [&](int c) {
-        if (!wait(bar(kBarKvFull + c % kStages), (c / kStages) & 1)) return;
+        if (!wait(bar(kBarKvFull + s_stage), s_parity)) return;
         tc_fence_after_sync();
-        const uint32_t k_tile = stage_k(c);
+        const uint64_t k = k_desc + (uint32_t)(s_stage * (kChunkBytes >> 4));
 #pragma unroll
-        for (int k = 0; k < kHeadDim / 16; ++k)
-          umma_bf16(tmem + 64 * (c & 1), umma_desc_sw128(sbase + 32 * k, 16, 1024),
-                    umma_desc_sw128(k_tile + 32 * k, 16, 1024), kIdS, k > 0);
+        for (int i = 0; i < kHeadDim / 16; ++i)
+          umma_bf16(tmem + 64 * (c & 1), q_desc + 2 * i, k + 2 * i, kIdS, i > 0);
         umma_commit(bar(kBarSFull + (c & 1)));
+        if (++s_stage == kStages) {
+          s_stage = 0;
+          s_parity ^= 1;
+        }
       };
       wait(q_full, 0);
       issue_s(0);
       if (n_chunks > 1) issue_s(1);
+      int stage = 0;
       for (int c = 0; ok && c < n_chunks; ++c) {
         // O_{c % 2} += P(c) V(c), 16 keys (one page of V, 8 columns of P) per
         // MMA; the first chunk of each side overwrites its accumulator.
         if (!wait(bar(kBarPFull + (c & 1)), (c >> 1) & 1)) break;
         tc_fence_after_sync();
-        const uint32_t v_tile = stage_k(c) + kKvBytes;
+        const uint64_t v = v_desc + (uint32_t)(stage * (kChunkBytes >> 4));
 #pragma unroll
-        for (int kk = 0; kk < kChunkPages; ++kk)
-          umma_bf16_ts(tmem + 128 + 64 * (c & 1), tmem + 64 * (c & 1) + 8 * kk,
-                       umma_desc_sw128(v_tile + kk * kTileBytes, 0, 1024), kIdO, (c >= 2 || kk > 0));
-        umma_commit(bar(kBarKvEmpty + c % kStages));
+        for (int i = 0; i < kChunkPages; ++i)
+          umma_bf16_ts(tmem + 128 + 64 * (c & 1), tmem + 64 * (c & 1) + 8 * i,
+                       v + (uint32_t)(i * (kTileBytes >> 4)), kIdO, (c >= 2 || i > 0));
+        umma_commit(bar(kBarKvEmpty + stage));
+        if (++stage == kStages) stage = 0;
         if (c + 2 < n_chunks) issue_s(c + 2);
       }
       if (ok) umma_commit(o_full);
@@ -372,8 +381,21 @@ __global__ void __launch_bounds__(kThreads, 2)
   const bool active = quarter < quarters;
   float m = -INFINITY, l = 0.f;  // this side's running max (base-2 units) and normaliser
   bool ok = true;
+  // The chunks that every row sees whole: those of pages [whole0, whole1), and
+  // those before page sinks_whole.
+  int whole0 = v_begin, whole1 = v_end, sinks_whole = 0;
+  if (!PREFIX) {
+    const long long low = (long long)pos_last + 1 - p.window;  // the last row sees from here on
+    const int first = low > 0 ? (int)((low + kPage - 1) / kPage) : 0;  // its first whole page
+    whole0 = max(span.head, first - span.skip);
+    if (span.skip == 0) whole0 = first;
+    whole1 = (pos0 + 1) / kPage - span.skip;
+    sinks_whole = min(span.head, p.sinks / kPage);
+  }
+  uint32_t parity = 0;
   for (int c = side; active && c < n_chunks; c += 2) {
-    bool ready = !*abort_flag && mbar_wait_bounded(bar(kBarSFull + side), (c >> 1) & 1);
+    bool ready = mbar_wait_bounded(bar(kBarSFull + side), parity);
+    parity ^= 1u;
     ready = __all_sync(0xffffffffu, ready);
     if (!ready) {
       if (lane == 0 && !*abort_flag) {
@@ -388,17 +410,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     tmem_ld32(tmem + 64 * side + lane_base, sr[0]);
     tmem_ld32(tmem + 64 * side + 32 + lane_base, sr[1]);
     tmem_wait_ld();
-    // Hidden keys: only chunks that are not seen whole by every row need the test.
     const int v0 = v_begin + c * kChunkPages;
-    bool whole = v0 + kChunkPages <= v_end;
-    if (!PREFIX) {
-#pragma unroll
-      for (int i = 0; i < kChunkPages; ++i) {
-        const int t0 = span.logical(v0 + i) * kPage;
-        whole = whole && t0 + kPage - 1 <= pos0 &&
-                ((long long)t0 > (long long)pos_last - p.window || t0 + kPage <= p.sinks);
-      }
-    }
+    const bool whole = (v0 >= whole0 && v0 + kChunkPages <= whole1) ||
+                       (!PREFIX && v0 + kChunkPages <= sinks_whole);
     if (!whole) {
 #pragma unroll
       for (int i = 0; i < kChunkPages; ++i) {
