@@ -14,15 +14,18 @@
 // Keys go in chunks of 4 pages (64 keys): warp 0 streams K and V boxes (TMA)
 // into a ring, one thread of warp 1 issues S = Q K^T and O += P V, two softmax
 // sides of four warps (one thread per row) take the chunks in turn, each with
-// its own S, P and O in Tensor Memory and its own running maximum and sum;
-// they merge at the end.  Unlike K3's, scores stay FP32, and P goes back into
-// the Tensor Memory columns of the scores it came from (two BF16 per column)
-// and is the MMA's A operand there: shared memory carries no P, whose write and
-// reads took half of its bandwidth (per 64-key chunk and tile 16 KB written and
-// 16 KB read, next to 24 KB for S, 8 KB for V and 16 KB from TMA).
-// The MMA thread issues S(0), S(1), then per chunk c: [wait P(c)] P V(c),
-// S(c + 2).  S(c)'s commit covers every earlier MMA, so when side c % 2 sees
-// S(c), P V(c - 2) has read P(c - 2), which S(c) overwrote, and written O.
+// its own P and O in Tensor Memory and its own running maximum and sum; they
+// merge at the end.  Unlike K3's, scores stay FP32, and P is written to Tensor
+// Memory (two BF16 per column) and is the MMA's A operand there: shared memory
+// carries no P, whose write and reads took half of its bandwidth (per 64-key
+// chunk and tile 16 KB written and 16 KB read, next to 24 KB for S, 8 KB for V
+// and 16 KB from TMA).
+// A side takes a chunk's scores into registers at once, so one S of 64 columns
+// serves both, and S(c + 2) is formed while chunk c is still in its
+// exponentials.  (With an S per side that P overwrote, S(c + 2) had to wait for
+// P V(c): a side idled 1000 of 3200 cycles per chunk.)  The MMA thread issues
+// S(0), then per chunk c: [wait: S(c) read] S(c + 1), [wait: P(c - 1) written]
+// P V(c - 1); a side waits for P V(c - 2) before it rescales its O or writes P(c).
 #include "tvp_span.cuh"
 #include "tvp_tile.cuh"
 #include "tvp_umma.cuh"
@@ -37,18 +40,22 @@ constexpr int kKvBytes = kChunkPages * kTileBytes;  // 8 KiB of K (or of V) per 
 constexpr int kChunkBytes = 2 * kKvBytes;
 constexpr int kQBytes = kRows * 128;
 constexpr int kThreads = 12 * 32;
-// S / P of side 0: 0-63, of side 1: 64-127; O of side 0: 128-191, of side 1: 192-255
+// S: columns 0-63; P of side 0: 64-95, of side 1: 96-127; O: 128-191 and 192-255
 constexpr uint32_t kTmemCols = 256;
+constexpr uint32_t kColP = 64, kColO = 128;
 constexpr int kLowRegs = 32;    // warps 0-3
 constexpr int kHighRegs = 104;  // the softmax warps
 constexpr int kMinChunks = 2;   // a piece of a prefix is no shorter than this
 
 constexpr int kOffStages = kQBytes;
 constexpr int kOffBars = kOffStages + kStages * kChunkBytes;
-// q_full, o_full, drain, (unused), s_full[2], p_full[2], kv_full[stages], kv_empty[stages]
+// q_full, o_full, drain, (unused), then by side: S formed, S read, P written, P V
+// done; kv_full[stages], kv_empty[stages]
 constexpr int kBarSFull = 4;
-constexpr int kBarPFull = 6;
-constexpr int kBarKvFull = 8;
+constexpr int kBarSRead = 6;
+constexpr int kBarPFull = 8;
+constexpr int kBarPvDone = 10;
+constexpr int kBarKvFull = 12;
 constexpr int kBarKvEmpty = kBarKvFull + kStages;
 constexpr int kNumBars = kBarKvEmpty + kStages;
 constexpr int kOffPlan = kOffBars + kNumBars * 8 + 16;
@@ -211,7 +218,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     mbar_init(drain, 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar(kBarSFull + b), 1);
+      mbar_init(bar(kBarSRead + b), quarters);
       mbar_init(bar(kBarPFull + b), quarters);
+      mbar_init(bar(kBarPvDone + b), 1);
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(bar(kBarKvFull + i), 1);
@@ -285,61 +294,76 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp == 1) {
     // ------------------------------ MMA issuer ----------------------------
-    if (lane == 0) {
-      constexpr uint32_t kIdS = umma_idesc_bf16_f32(kRows, kChunk, false, false);
-      constexpr uint32_t kIdO = umma_idesc_bf16_f32(kRows, kHeadDim, false, true);
-      // Descriptors of Q and of stage 0's K and V; a byte offset adds offset / 16.
-      const uint64_t q_desc = umma_desc_sw128(sbase, 16, 1024);
-      const uint64_t k_desc = umma_desc_sw128(sbase + kOffStages, 16, 1024);
-      const uint64_t v_desc = umma_desc_sw128(sbase + kOffStages + kKvBytes, 0, 1024);
-      bool ok = true;
-      auto wait = [&](uint32_t b, uint32_t parity) {
-        if (ok && !mbar_wait_bounded(b, parity)) {
-          record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_FULL);
-          ok = false;
-        }
-        return ok;
-      };
-      // S(c) = Q K(c)^T into the columns of side c % 2, 16 channels per MMA.
-      int s_stage = 0, s_parity = 0;  // of the next chunk of S
-      auto issue_s = [&](int c) {
-        if (!wait(bar(kBarKvFull + s_stage), s_parity)) return;
-        tc_fence_after_sync();
-        const uint64_t k = k_desc + (uint32_t)(s_stage * (kChunkBytes >> 4));
+    // The whole warp waits and works out the operands, one lane issues.
+    constexpr uint32_t kIdS = umma_idesc_bf16_f32(kRows, kChunk, false, false);
+    constexpr uint32_t kIdO = umma_idesc_bf16_f32(kRows, kHeadDim, false, true);
+    const uint32_t cols = __shfl_sync(0xffffffffu, tmem, 0);
+    const int chunks = __shfl_sync(0xffffffffu, n_chunks, 0);
+    // Descriptors of Q and of stage 0's K and V; a byte offset adds offset / 16.
+    const uint64_t q_desc = umma_desc_sw128(sbase, 16, 1024);
+    const uint64_t k_desc = umma_desc_sw128(sbase + kOffStages, 16, 1024);
+    const uint64_t v_desc = umma_desc_sw128(sbase + kOffStages + kKvBytes, 0, 1024);
+    bool ok = true;
+    auto wait = [&](uint32_t b, uint32_t parity) {
+      if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(b, parity))) {
+        if (lane == 0) record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_FULL);
+        ok = false;
+      }
+      return ok;
+    };
+    // S(c) = Q K(c)^T, 16 channels per MMA, for side c % 2.
+    int s_stage = 0, s_parity = 0;  // of the next chunk of S
+    auto issue_s = [&](int c) {
+      if (!wait(bar(kBarKvFull + s_stage), s_parity)) return;
+      tc_fence_after_sync();
+      const uint64_t k = k_desc + (uint32_t)(s_stage * (kChunkBytes >> 4));
+      if (elect_one()) {
 #pragma unroll
         for (int i = 0; i < kHeadDim / 16; ++i)
-          umma_bf16(tmem + 64 * (c & 1), q_desc + 2 * i, k + 2 * i, kIdS, i > 0);
+          umma_bf16(cols, q_desc + 2 * i, k + 2 * i, kIdS, i > 0);
         umma_commit(bar(kBarSFull + (c & 1)));
-        if (++s_stage == kStages) {
-          s_stage = 0;
-          s_parity ^= 1;
-        }
-      };
-      wait(q_full, 0);
-      issue_s(0);
-      if (n_chunks > 1) issue_s(1);
-      int stage = 0;
-      for (int c = 0; ok && c < n_chunks; ++c) {
-        // O_{c % 2} += P(c) V(c), 16 keys (one page of V, 8 columns of P) per
-        // MMA; the first chunk of each side overwrites its accumulator.
-        if (!wait(bar(kBarPFull + (c & 1)), (c >> 1) & 1)) break;
-        tc_fence_after_sync();
-        const uint64_t v = v_desc + (uint32_t)(stage * (kChunkBytes >> 4));
+      }
+      __syncwarp();
+      if (++s_stage == kStages) {
+        s_stage = 0;
+        s_parity ^= 1;
+      }
+    };
+    wait(q_full, 0);
+    issue_s(0);
+    int stage = 0;
+    for (int c = 0; ok && c <= chunks; ++c) {
+      if (c + 1 < chunks) {  // S(c) is in the registers of its side
+        if (!wait(bar(kBarSRead + (c & 1)), (c >> 1) & 1)) break;
+        issue_s(c + 1);
+      }
+      if (c == 0) continue;
+      // O_s += P(d) V(d) for d = c - 1 and its side s, 16 keys (one page of V, 8
+      // columns of P) per MMA; the first chunk of each side overwrites O.
+      const int d = c - 1, side = d & 1;
+      if (!wait(bar(kBarPFull + side), (d >> 1) & 1)) break;
+      tc_fence_after_sync();
+      const uint64_t v = v_desc + (uint32_t)(stage * (kChunkBytes >> 4));
+      if (elect_one()) {
 #pragma unroll
         for (int i = 0; i < kChunkPages; ++i)
-          umma_bf16_ts(tmem + 128 + 64 * (c & 1), tmem + 64 * (c & 1) + 8 * i,
-                       v + (uint32_t)(i * (kTileBytes >> 4)), kIdO, (c >= 2 || i > 0));
+          umma_bf16_ts(cols + kColO + 64 * side, cols + kColP + 32 * side + 8 * i,
+                       v + (uint32_t)(i * (kTileBytes >> 4)), kIdO, (d >= 2 || i > 0));
+        umma_commit(bar(kBarPvDone + side));
         umma_commit(bar(kBarKvEmpty + stage));
-        if (++stage == kStages) stage = 0;
-        if (c + 2 < n_chunks) issue_s(c + 2);
       }
+      __syncwarp();
+      if (++stage == kStages) stage = 0;
+    }
+    if (!ok && lane == 0) *abort_flag = 1;
+    if (elect_one()) {
       if (ok) umma_commit(o_full);
-      if (!ok) *abort_flag = 1;
       // Every MMA issued has completed before Tensor Memory is released.
       umma_commit(drain);
-      if (!mbar_wait_bounded(drain, 0))
-        record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_DRAIN);
     }
+    __syncwarp();
+    if (!__all_sync(0xffffffffu, mbar_wait_bounded(drain, 0)) && lane == 0)
+      record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_DRAIN);
     __syncwarp();
     tc_fence_before_sync();
     named_barrier_sync(1, kEndThreads);
@@ -392,24 +416,32 @@ __global__ void __launch_bounds__(kThreads, 2)
     whole1 = (pos0 + 1) / kPage - span.skip;
     sinks_whole = min(span.head, p.sinks / kPage);
   }
-  uint32_t parity = 0;
-  for (int c = side; active && c < n_chunks; c += 2) {
-    bool ready = mbar_wait_bounded(bar(kBarSFull + side), parity);
-    parity ^= 1u;
-    ready = __all_sync(0xffffffffu, ready);
-    if (!ready) {
-      if (lane == 0 && !*abort_flag) {
-        *abort_flag = 1;
-        record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_FULL);
-      }
-      ok = false;
-      break;
+  // A wait of the whole warp, after a test of the barrier made earlier (a wait
+  // costs some 250 cycles of latency even when there is nothing to wait for);
+  // false when it ran out.
+  auto warp_wait = [&](uint32_t b, uint32_t parity, bool tested) {
+    if (__all_sync(0xffffffffu, tested)) return true;
+    if (__all_sync(0xffffffffu, mbar_wait_bounded(b, parity))) return true;
+    if (lane == 0 && !*abort_flag) {
+      *abort_flag = 1;
+      record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_FULL);
     }
+    return false;
+  };
+  uint32_t parity = 0;
+  bool s_formed = false, pv_done = false;
+  for (int c = side; active && c < n_chunks; c += 2) {
+    ok = warp_wait(bar(kBarSFull + side), parity, s_formed);
+    if (!ok) break;
     tc_fence_after_sync();
     uint32_t sr[2][32];
-    tmem_ld32(tmem + 64 * side + lane_base, sr[0]);
-    tmem_ld32(tmem + 64 * side + 32 + lane_base, sr[1]);
+    tmem_ld32(tmem + lane_base, sr[0]);
+    tmem_ld32(tmem + 32 + lane_base, sr[1]);
+    if (c >= 2) pv_done = mbar_test(bar(kBarPvDone + side), parity ^ 1u);
     tmem_wait_ld();
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(kBarSRead + side));
     const int v0 = v_begin + c * kChunkPages;
     const bool whole = (v0 >= whole0 && v0 + kChunkPages <= whole1) ||
                        (!PREFIX && v0 + kChunkPages <= sinks_whole);
@@ -444,12 +476,16 @@ __global__ void __launch_bounds__(kThreads, 2)
       alpha = m == -INFINITY ? 0.f : fast_exp2(m - top);
       m = top;
     }
+    if (c >= 2) {  // P V(c - 2) is the last MMA into this side's O and out of its P
+      ok = warp_wait(bar(kBarPvDone + side), parity ^ 1u, pv_done);
+      if (!ok) break;
+      tc_fence_after_sync();
+    }
+    parity ^= 1u;
     if (c >= 2 && __any_sync(0xffffffffu, alpha != 1.f)) {
-      // O_side holds this side's earlier chunks: S(c)'s commit, just waited
-      // for, covered P V(c - 2), the last MMA into it.
 #pragma unroll 1
       for (int part = 0; part < 4; ++part) {
-        const uint32_t taddr = tmem + 128 + 64 * side + 16 * part + lane_base;
+        const uint32_t taddr = tmem + kColO + 64 * side + 16 * part + lane_base;
         uint32_t o[16];
         tmem_ld16(taddr, o);
         tmem_wait_ld();
@@ -463,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint64_t ls2[4];  // four independent paired sums
 #pragma unroll
     for (int i = 0; i < 4; ++i) ls2[i] = f2_pack(0.f, 0.f);
-    // P over the scores' own columns, two keys per column.
+    // P, two keys per column.
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       uint32_t w[16];
@@ -478,8 +514,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         ls2[j & 3] = f2_add(ls2[j & 3], f2_pack(p0, p1));
         w[j] = pack_bf16x2(p0, p1);
       }
-      tmem_st16(tmem + 64 * side + 16 * half + lane_base, w);
+      tmem_st16(tmem + kColP + 32 * side + 16 * half + lane_base, w);
     }
+    s_formed = mbar_test(bar(kBarSFull + side), parity);  // of this side's next chunk
     tmem_wait_st();
     float la, lb;
     f2_unpack(f2_add(f2_add(ls2[0], ls2[1]), f2_add(ls2[2], ls2[3])), la, lb);
@@ -502,12 +539,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(kBarPFull + side));
   }
-  bool fin = active && ok && !*abort_flag && mbar_wait_bounded(o_full, 0);
-  fin = __all_sync(0xffffffffu, fin);
-  if (active && !fin && ok && lane == 0 && !*abort_flag) {
-    *abort_flag = 1;
-    record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_FULL);
-  }
+  const bool fin = active && ok && warp_wait(o_full, 0, false);
   // Merge the two sides per row: side 1 hands its (max, normaliser) to side 0
   // through the Q tile, whose last reader (an S MMA) completed before o_full.
   float* xchg = reinterpret_cast<float*>(smem);
@@ -533,8 +565,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       uint32_t oa[32], ob[32];
-      tmem_ld32(tmem + 128 + 32 * half + lane_base, oa);
-      if (two) tmem_ld32(tmem + 192 + 32 * half + lane_base, ob);
+      tmem_ld32(tmem + kColO + 32 * half + lane_base, oa);
+      if (two) tmem_ld32(tmem + kColO + 64 + 32 * half + lane_base, ob);
       tmem_wait_ld();
       if (!valid) continue;
       float x[32];

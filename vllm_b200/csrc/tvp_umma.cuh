@@ -34,6 +34,19 @@ __device__ __forceinline__ void tc_fence_after_sync() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
+// True in one lane of a converged warp.  An MMA's operands come from uniform
+// registers: a warp that works them out together and lets one lane issue has
+// them there, where a single thread's must be moved one by one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p)::"memory");
+  return p != 0;
+}
+
 // ---- shared-memory matrix descriptor --------------------------------------
 // Bits [0,14) start address >> 4, [16,30) leading byte offset >> 4, [32,46)
 // stride byte offset >> 4, [46,48) version (1 on sm_100), [49,52) base
