@@ -451,8 +451,7 @@ int tvp_paged_window_decode_attention(const tvp_bf16* q, const tvp_bf16* k_pool,
  * its first d_seq_lens[b] tokens.  A row of length 0 gets zeros; one shorter
  * than its prefix gets zeros and TVP_DEVERR_BAD_LENGTH.  Group rows that are
  * out of order set TVP_DEVERR_BAD_PLAN and nothing is written.  groups = 0 is
- * plain decode attention.  Two launches on `stream`; what a call right before
- * may write while it releases its dependents early is as for K6.
+ * plain decode attention.  Three launches on `stream`.
  */
 int tvp_paged_shared_prefix_decode_attention(
     const tvp_bf16* q, const tvp_bf16* k_pool, const tvp_bf16* v_pool, int num_pages,

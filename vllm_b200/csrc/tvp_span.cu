@@ -25,19 +25,21 @@ bool span_heads_supported(int kv_heads) {
 }
 
 struct SpanWorkspace {
-  size_t group_pieces, partials, pieces, total;
+  size_t row_ranges, group_pieces, partials, pieces, total;
   int max_pieces;
 };
 
-// counters[1024][8] | group_pieces[groups] | partials[2 num_ctas][kv_heads] | pieces.
+// counters[1024][8] | row_ranges[batch] | group_pieces[groups] | partials | pieces.
 // The counters' place and size are the same for every call.  Pieces: two CTAs
 // per SM, or one per tile of 32 rows and KV head where those are more.
 SpanWorkspace span_workspace(int batch, int groups, int kv_heads, int num_ctas) {
   auto align = [](size_t x) { return (x + 255) / 256 * 256; };
   SpanWorkspace w = {};
-  w.group_pieces = (size_t)kMaxSpanCtas * kMaxKvHeads * 4;
+  w.row_ranges = (size_t)kMaxSpanCtas * kMaxKvHeads * 4;
+  w.group_pieces = w.row_ranges + (groups > 0 ? align((size_t)batch * sizeof(int2)) : 0);
   w.partials = align(w.group_pieces + (size_t)groups * sizeof(int2));
-  w.pieces = align(w.partials + (size_t)num_ctas * 2 * kv_heads * kPartialFloats * 4);
+  const size_t slots = groups > 0 ? (size_t)batch + num_ctas : (size_t)2 * num_ctas;
+  w.pieces = align(w.partials + slots * kv_heads * kPartialFloats * 4);
   if (groups > 0) {
     const int streams = kv_heads * (batch / kTileRows + groups);
     w.max_pieces = streams > 2 * num_ctas ? streams : 2 * num_ctas;
@@ -67,6 +69,7 @@ void fill_span(const tvp_bf16* q, const tvp_bf16* k_pool, const tvp_bf16* v_pool
 void fill_workspace(void* d_workspace, const SpanWorkspace& w, int num_ctas, SpanParams* p) {
   char* base = static_cast<char*>(d_workspace);
   p->counters = reinterpret_cast<int32_t*>(base);
+  p->row_ranges = reinterpret_cast<int2*>(base + w.row_ranges);
   p->group_pieces = reinterpret_cast<int2*>(base + w.group_pieces);
   p->partials = reinterpret_cast<float*>(base + w.partials);
   p->pieces = reinterpret_cast<float*>(base + w.pieces);
@@ -150,9 +153,10 @@ int tvp_paged_shared_prefix_decode_attention(
   fill_workspace(d_workspace, w, ctas, &p);
   const long long rows = (long long)num_layers * num_pages * kPage;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (groups > 0 && (rc = map_cuda(launch_prefix_tiles(p, rows, w.max_pieces, st))) != TVP_OK)
+  if ((rc = map_cuda(launch_span_decode(p, groups > 0, rows, ctas, st))) != TVP_OK || groups == 0)
     return rc;
-  return map_cuda(launch_span_decode(p, groups > 0, rows, ctas, st));
+  if ((rc = map_cuda(launch_prefix_tiles(p, rows, w.max_pieces, st))) != TVP_OK) return rc;
+  return map_cuda(launch_prefix_merge(p, st));
 }
 
 int tvp_paged_window_prefill_attention(const tvp_bf16* q, const tvp_bf16* k_pool,

@@ -33,7 +33,10 @@ struct SpanParams {
   int32_t* err;
   // workspace
   int32_t* counters;   // [kMaxSpanCtas][8]: arrivals of the row that starts in a range and leaves it
-  float* partials;     // [2 ctas][kv_heads] split-K partials
+  float* partials;     // split-K partials: [2 ctas][kv_heads], or, of rows with prefixes,
+                       // [row + range][kv_heads]
+  // rows with prefixes
+  int2* row_ranges;    // [batch]: first and last range of a row's own pages
   int2* group_pieces;  // [groups]: first piece, pieces per (tile, KV head)
   float* pieces;       // [piece][row of the tile] partials of the shared prefixes
   int piece_target;    // pieces to aim at
@@ -129,6 +132,7 @@ cudaError_t launch_span_decode(const SpanParams& p, bool shared, long long pool_
                                cudaStream_t stream);
 cudaError_t launch_prefix_tiles(const SpanParams& p, long long pool_rows, int max_pieces,
                                 cudaStream_t stream);
+cudaError_t launch_prefix_merge(const SpanParams& p, cudaStream_t stream);
 cudaError_t launch_window_tiles(const SpanParams& p, long long pool_rows, int max_q_len,
                                 int num_seqs, cudaStream_t stream);
 

@@ -9,8 +9,10 @@
 //     recomputes each row's span from its length.  One load of the lengths and a
 //     block scan replace a launch per step, about 2.5 us, which is what a small
 //     batch takes altogether.
-//   * SHARED: a finished row also merges the pieces of its group's prefix that
-//     the tile kernel left, through one (m, l, O) fold per piece.
+//   * SHARED: a row's pieces are left as partials, which the merge kernel folds
+//     together with the pieces of its group's prefix.  The CTA is half as large
+//     (8 consumer warps, 4 stages), so that a CTA of the tile kernel shares the SM
+//     with it: this kernel waits for HBM, that one for its exponentials.
 //
 // Bound by HBM: each visible token's K and V are read once (2 KiB for 8 heads).
 // A row that is cut by ranges counts its pieces at the range it starts in: at
@@ -22,12 +24,24 @@
 namespace tvp {
 namespace {
 
-constexpr int kStages = 6;
 constexpr int kTailBarrier = 14;  // the 16 consumer warps, before the stages become merge scratch
-constexpr size_t kBarsAt = (size_t)kStages * kStageBytes;
-constexpr size_t kScratchAt = (kBarsAt + 2 * kStages * 8 + (kStages + 4) * 4 + 15) / 16 * 16;
-constexpr size_t kSetupAt = kScratchAt + (size_t)kMergeSlots * kStateFloats * 32 * 4;
-constexpr size_t kSpanSmem = kSetupAt + 256;
+
+// Shape and shared memory of a CTA.
+template <int KVH, bool SHARED>
+struct Shape {
+  static constexpr int kSets = SHARED ? 1 : 2;  // of 8 consumer warps
+  static constexpr int kStages = SHARED ? 4 : 6;
+  static constexpr int kThreads = decode_threads<kSets, true>();
+  // Registers: SHARED leaves the tile kernel's CTA its 30,720.
+  static constexpr int kBlocks = SHARED ? 2 : 1;
+  static constexpr int kConsumer = SHARED ? 96 : kConsumerRegs;
+  static constexpr int kWays = kSets * kStageTiles / KVH;
+  static constexpr size_t kBarsAt = (size_t)kStages * kStageBytes;
+  static constexpr size_t kScratchAt = (kBarsAt + 2 * kStages * 8 + (kStages + 4) * 4 + 15) / 16 * 16;
+  // senders of the widest merge level: kWays / 2 of each head
+  static constexpr size_t kSetupAt = kScratchAt + (size_t)(kWays / 2 * KVH) * kStateFloats * 32 * 4;
+  static constexpr size_t kSmem = kSetupAt + 256;
+};
 
 // Fold of one partial into this lane's (m, l, 8 channels) of a query head.
 struct Fold {
@@ -43,21 +57,26 @@ struct Fold {
     o[4] = o[4] * wa + b.x * wb; o[5] = o[5] * wa + b.y * wb;
     o[6] = o[6] * wa + b.z * wb; o[7] = o[7] * wa + b.w * wb;
   }
-  // n partials, the i-th at at(i), two in flight at once, folded in order.
+  // n partials, the i-th at at(i), kFlight in flight at once, folded in order.
+  static constexpr int kFlight = 6;
   template <typename At>
   __device__ __forceinline__ void add_all(int n, At at, int lane) {
     const int h = lane >> 3, d = 2 * kGroup + h * kHeadDim + (lane & 7) * 8;
-    for (int i = 0; i < n; i += 2) {
-      const float* x = at(i);
-      const float* y = i + 1 < n ? at(i + 1) : x;
-      const float xm = __ldcg(x + h), xl = __ldcg(x + kGroup + h);
-      const float ym = __ldcg(y + h), yl = __ldcg(y + kGroup + h);
-      const float4 xa = __ldcg(reinterpret_cast<const float4*>(x + d));
-      const float4 xb = __ldcg(reinterpret_cast<const float4*>(x + d + 4));
-      const float4 ya = __ldcg(reinterpret_cast<const float4*>(y + d));
-      const float4 yb = __ldcg(reinterpret_cast<const float4*>(y + d + 4));
-      add(xm, xl, xa, xb);
-      if (i + 1 < n) add(ym, yl, ya, yb);
+    for (int i = 0; i < n; i += kFlight) {
+      float pm[kFlight], pl[kFlight];
+      float4 a[kFlight], b[kFlight];
+#pragma unroll
+      for (int e = 0; e < kFlight; ++e) {
+        if (i + e >= n) continue;
+        const float* x = at(i + e);
+        pm[e] = __ldcg(x + h);
+        pl[e] = __ldcg(x + kGroup + h);
+        a[e] = __ldcg(reinterpret_cast<const float4*>(x + d));
+        b[e] = __ldcg(reinterpret_cast<const float4*>(x + d + 4));
+      }
+#pragma unroll
+      for (int e = 0; e < kFlight; ++e)
+        if (i + e < n) add(pm[e], pl[e], a[e], b[e]);
     }
   }
   __device__ __forceinline__ void write(__nv_bfloat16* out, int lane) const {
@@ -71,40 +90,32 @@ struct Fold {
   }
 };
 
-// The pieces of row s's shared prefix for KV head h, folded into f.
-template <int KVH>
-__device__ __forceinline__ void fold_prefix(const SpanParams& p, Fold& f, int s, int h, int lane) {
-  const int g = group_of(p, s);
-  if (g < 0) return;
-  const int2 at = __ldcg(p.group_pieces + g);  // written by the launch before
-  const int t = s - __ldg(p.group_rows + g);
-  const float* base = p.pieces +
-                      ((size_t)(at.x + ((t / kTileRows) * KVH + h) * at.y) * kTileRows +
-                       t % kTileRows) * kPartialFloats;
-  f.add_all(at.y, [&](int i) { return base + (size_t)i * kPieceFloats; }, lane);
-}
-
 template <int KVH, bool SHARED>
-__global__ void __launch_bounds__(decode_threads<2, true>(), 1)
+__global__ void __launch_bounds__(Shape<KVH, SHARED>::kThreads, Shape<KVH, SHARED>::kBlocks)
     span_decode_kernel(const SpanParams p, const __grid_constant__ CUtensorMap k_map,
                        const __grid_constant__ CUtensorMap v_map) {
-  constexpr int PS = kStageTiles / KVH;  // pages per stage
-  constexpr int PERIOD = 2 * PS;         // pages between two pages of one way
+  using Cta = Shape<KVH, SHARED>;
+  constexpr int kStages = Cta::kStages;
+  constexpr int PS = kStageTiles / KVH;      // pages per stage
+  constexpr int PERIOD = Cta::kSets * PS;    // pages between two pages of one way
+  constexpr int kConsumers = Cta::kSets * kStageTiles;
   // 1 KiB alignment of the stage tiles (128-byte swizzle); checked, as in K2.
   extern __shared__ __align__(1024) unsigned char smem[];
   if (smem_addr(smem) & 1023u) {
     if (threadIdx.x == 0) record_error(p.err, TVP_DEVERR_SMEM_ALIGN);
     return;
   }
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kBarsAt);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cta::kBarsAt);
   uint64_t* empty_bar = full_bar + kStages;
   int* stage_mask = reinterpret_cast<int*>(empty_bar + kStages);  // bit o: page o of the stage loaded
   volatile int* abort_flag = stage_mask + kStages;
-  float* scratch = reinterpret_cast<float*>(smem + kScratchAt);
-  int* warp_sums = reinterpret_cast<int*>(smem + kSetupAt);     // [warps]
-  int* start = reinterpret_cast<int*>(smem + kSetupAt + 128);  // row and its first page
+  float* scratch = reinterpret_cast<float*>(smem + Cta::kScratchAt);
+  int* warp_sums = reinterpret_cast<int*>(smem + Cta::kSetupAt);     // [warps]
+  int* start = reinterpret_cast<int*>(smem + Cta::kSetupAt + 128);  // row and its first page
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // The tile kernel may start beside this one.
+  if (SHARED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (SHARED && !groups_in_order(p)) {
     if (tid == 0 && blockIdx.x == 0) record_error(p.err, TVP_DEVERR_BAD_PLAN);
     return;
@@ -156,10 +167,10 @@ __global__ void __launch_bounds__(decode_threads<2, true>(), 1)
   __syncthreads();
   const uint32_t smem_base = smem_addr(smem);
 
-  if (warp >= 2 * kStageTiles) {
+  if (warp >= kConsumers) {
     // ------------------------------ producer ------------------------------
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
-    if (warp != 2 * kStageTiles) return;
+    if (warp != kConsumers) return;
     if (lane == 0) {
       prefetch_tensor_map(&k_map);
       prefetch_tensor_map(&v_map);
@@ -185,8 +196,7 @@ __global__ void __launch_bounds__(decode_threads<2, true>(), 1)
     }
     // Launched as a programmatic dependent launch: the kernel before may still
     // run.  It writes pages and q, never lengths or tables, so the walk starts
-    // now and the wait comes before the first copy.  (SHARED: that kernel is
-    // the tile kernel, which only reads what this one copies.)
+    // now and the wait comes before the first copy.  (SHARED starts after it.)
     if (!SHARED) {
       asm volatile("griddepcontrol.wait;" ::: "memory");
       asm volatile("fence.proxy.async.global;" ::: "memory");
@@ -244,14 +254,8 @@ __global__ void __launch_bounds__(decode_threads<2, true>(), 1)
   }
 
   // ------------------------------ consumers -------------------------------
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
-  // SHARED waits where it first needs the prefix's pieces.
-  bool waited = false;
-  auto wait_for_previous = [&]() {
-    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
-    waited = true;
-  };
-  if (!SHARED) wait_for_previous();
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cta::kConsumer));
+  if (!SHARED) asm volatile("griddepcontrol.wait;" ::: "memory");
   const int set = warp / kStageTiles;
   const int t = warp % kStageTiles;  // tile of the stage this warp reads
   const int o = t / KVH, h = t % KVH;
@@ -322,90 +326,92 @@ __global__ void __launch_bounds__(decode_threads<2, true>(), 1)
                                (keep >> (tl.tr + 8)) & 1u, p.scale_log2);
     }
 
-    merge_ways<KVH>(st, scratch, way, h, lane);
-    if (piece_end == p_end && !complete) {
-      last_partial = true;  // published and merged below
-      break;
-    }
-    if (way == 0) {
-      reduce_l(st);
-      const int r0 = range_of_page(first, T, C);
-      const int pieces = range_of_page(end - 1, T, C) - r0 + 1;
-      float* part = p.partials + ((size_t)partial_slot((int)c, first, T, C) * KVH + h) * kPartialFloats;
-      int32_t* counter = p.counters + r0 * kMaxKvHeads + h;
-      if (SHARED) {
-        // This warp's own merge slot, which the next piece's entry barrier guards.
-        float* row = scratch + (size_t)h * kStateFloats * 32;
-        bool last = true;
+    merge_ways<KVH, Cta::kWays>(st, scratch, way, h, lane);
+    const int r0 = range_of_page(first, T, C), r1 = range_of_page(end - 1, T, C);
+    if (SHARED) {
+      if (way == 0) {
+        reduce_l(st);
+        // row + range: each next piece raises one of them
+        write_partial(st, p.partials + ((size_t)(s + c) * KVH + h) * kPartialFloats, tl);
+        if (pg == first && h == 0 && lane == 0) p.row_ranges[s] = make_int2(r0, r1);
+      }
+    } else {
+      if (piece_end == p_end && !complete) {
+        last_partial = true;  // published and merged below
+        break;
+      }
+      if (way == 0) {
+        reduce_l(st);
         if (complete)
-          write_partial(st, row, tl);
-        else
-          last = publish_partial_at(st, part, counter, pieces, tl, lane);
-        __syncwarp();
-        if (last) {
-          Fold f;
-          if (complete) {
-            const int d = 2 * kGroup + (lane >> 3) * kHeadDim + (lane & 7) * 8;
-            f.add(row[lane >> 3], row[kGroup + (lane >> 3)], *reinterpret_cast<float4*>(row + d),
-                  *reinterpret_cast<float4*>(row + d + 4));
-          } else {
-            f.add_all(pieces, [&](int i) { return partial_of(p.partials, KVH, h, r0 + i, r0, first, T, C); },
-                      lane);
-          }
-          wait_for_previous();
-          fold_prefix<KVH>(p, f, s, h, lane);
-          f.write(out_of(s), lane);
-        }
-        __syncwarp();
-      } else if (complete) {
-        write_output(st, local_out(out_of(s)), tl);
-      } else if (publish_partial_at(st, part, counter, pieces, tl, lane)) {
-        combine_partials<1>(p.partials, KVH, h, first, end, T, C, local_out(out_of(s)), lane);
+          write_output(st, local_out(out_of(s)), tl);
+        else if (publish_partial_at(
+                     st, p.partials + ((size_t)partial_slot((int)c, first, T, C) * KVH + h) * kPartialFloats,
+                     p.counters + r0 * kMaxKvHeads + h, r1 - r0 + 1, tl, lane))
+          combine_partials<1>(p.partials, KVH, h, first, end, T, C, local_out(out_of(s)), lane);
       }
     }
     kbase += np;
     pg = piece_end;
   }
+  if (SHARED) return;
   if (last_partial) {
     // The range's last piece ends inside a row that started earlier: once every
     // consumer warp has read its last tile the stages are free, and head h's
     // share of them holds the row's partials for the merge (K2h).
-    named_barrier_sync(kTailBarrier, 2 * kStageTiles * 32);
+    named_barrier_sync(kTailBarrier, kConsumers * 32);
     if (way == 0) {
       reduce_l(st);
       const int end = first + span.pages;
       const int r0 = range_of_page(first, T, C);
-      const int pieces = range_of_page(end - 1, T, C) - r0 + 1;
       if (publish_partial_at(
               st, p.partials + ((size_t)partial_slot((int)c, first, T, C) * KVH + h) * kPartialFloats,
-              p.counters + r0 * kMaxKvHeads + h, pieces, tl, lane)) {
-        if (SHARED) {
-          Fold f;
-          f.add_all(pieces, [&](int i) { return partial_of(p.partials, KVH, h, r0 + i, r0, first, T, C); },
-                    lane);
-          wait_for_previous();
-          fold_prefix<KVH>(p, f, s, h, lane);
-          f.write(out_of(s), lane);
-        } else {
-          constexpr int kShareBytes = kStages * kStageBytes / KVH;
-          combine_partials_staged(p.partials, KVH, h, first, end, T, C, local_out(out_of(s)), lane,
-                                  reinterpret_cast<float*>(smem + (size_t)h * kShareBytes),
-                                  (kShareBytes - 512) / 1024);
-        }
+              p.counters + r0 * kMaxKvHeads + h, range_of_page(end - 1, T, C) - r0 + 1, tl, lane)) {
+        constexpr int kShareBytes = kStages * kStageBytes / KVH;
+        combine_partials_staged(p.partials, KVH, h, first, end, T, C, local_out(out_of(s)), lane,
+                                reinterpret_cast<float*>(smem + (size_t)h * kShareBytes),
+                                (kShareBytes - 512) / 1024);
       }
     }
   }
-  // Rows without pages of their own: nothing, or the shared prefix alone.
+  // Rows without pages attend to nothing.
   if (way == 0) {
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-      const RowSpan r = decode_span<SHARED>(p, b, false);
-      if (r.pages > 0) continue;
-      wait_for_previous();
-      Fold f;
-      if (SHARED && r.len > 0) fold_prefix<KVH>(p, f, b, h, lane);
-      f.write(out_of(b), lane);
-    }
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
+      if (decode_span<SHARED>(p, b, false).pages == 0)
+        *reinterpret_cast<uint4*>(out_of(b) + lane * 8) = make_uint4(0, 0, 0, 0);
   }
+}
+
+// The last step of K7: a warp per (row, KV head) folds the partials of the row's
+// own pages and of its group's prefix, and writes the output; all of them read
+// from L2, a few microseconds for any batch.  (Folded by the decode kernel's
+// warps as they finished a row, the prefix pieces cost 2 to 3 us per row there,
+// with the pipeline standing.)
+constexpr int kMergeWarps = 8;
+
+template <int KVH>
+__global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const SpanParams p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool in_order = groups_in_order(p);
+  const int s = blockIdx.x * (kMergeWarps / KVH) + warp / KVH, h = warp % KVH;
+  if (!in_order || s >= p.batch) return;
+  // What the call's inputs say, before the launches before this one are done.
+  const RowSpan span = decode_span<true>(p, s, false);
+  const int g = span.len > 0 ? group_of(p, s) : -1;
+  const int t = g >= 0 ? s - __ldg(p.group_rows + g) : 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  Fold f;
+  if (g >= 0) {
+    const int2 at = __ldcg(p.group_pieces + g);
+    const float* base = p.pieces + ((size_t)(at.x + ((t / kTileRows) * KVH + h) * at.y) * kTileRows +
+                                    t % kTileRows) * kPartialFloats;
+    f.add_all(at.y, [&](int i) { return base + (size_t)i * kPieceFloats; }, lane);
+  }
+  if (span.pages > 0) {
+    const int2 r = __ldcg(p.row_ranges + s);
+    const float* base = p.partials + ((size_t)(s + r.x) * KVH + h) * kPartialFloats;
+    f.add_all(r.y - r.x + 1, [&](int i) { return base + (size_t)i * KVH * kPartialFloats; }, lane);
+  }
+  f.write(p.out + ((size_t)s * KVH + h) * kGroup * kHeadDim, lane);
 }
 
 template <int KVH, bool SHARED>
@@ -420,22 +426,25 @@ cudaError_t launch(const SpanParams& p, const CUtensorMap& k_map, const CUtensor
     cudaFuncAttributes fa;
     e = cudaFuncGetAttributes(&fa, span_decode_kernel<KVH, SHARED>);
     if (e != cudaSuccess) return e;
-    if (!regsplit_fits(fa.numRegs, decode_threads<2, true>())) return cudaErrorInvalidConfiguration;
+    constexpr int kThreads = Shape<KVH, SHARED>::kThreads;
+    if (fa.numRegs * kThreads < 128 * kProducerRegs + (kThreads - 128) * Shape<KVH, SHARED>::kConsumer)
+      return cudaErrorInvalidConfiguration;
     e = cudaFuncSetAttribute(span_decode_kernel<KVH, SHARED>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSpanSmem);
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)Shape<KVH, SHARED>::kSmem);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)num_ctas);
-  cfg.blockDim = dim3(decode_threads<2, true>());
-  cfg.dynamicSmemBytes = kSpanSmem;
+  cfg.blockDim = dim3(Shape<KVH, SHARED>::kThreads);
+  cfg.dynamicSmemBytes = Shape<KVH, SHARED>::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = SHARED ? 0 : 1;  // SHARED: the tile kernel beside it counts on a full wait here
   return cudaLaunchKernelEx(&cfg, span_decode_kernel<KVH, SHARED>, p, k_map, v_map);
 }
 
@@ -451,7 +460,31 @@ cudaError_t launch_heads(const SpanParams& p, const CUtensorMap& k_map, const CU
   }
 }
 
+template <int KVH>
+cudaError_t launch_merge(const SpanParams& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.batch + kMergeWarps / KVH - 1) / (kMergeWarps / KVH)));
+  cfg.blockDim = dim3(kMergeWarps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, prefix_merge_kernel<KVH>, p);
+}
+
 }  // namespace
+
+cudaError_t launch_prefix_merge(const SpanParams& p, cudaStream_t stream) {
+  switch (p.kv_heads) {
+    case 1: return launch_merge<1>(p, stream);
+    case 2: return launch_merge<2>(p, stream);
+    case 4: return launch_merge<4>(p, stream);
+    case 8: return launch_merge<8>(p, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
 
 cudaError_t launch_span_decode(const SpanParams& p, bool shared, long long pool_rows, int num_ctas,
                                cudaStream_t stream) {

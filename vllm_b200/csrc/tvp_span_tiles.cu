@@ -3,7 +3,7 @@
 // pages, 128 MMA rows 4 t + h, so every K/V byte serves 4 heads of 32 tokens.
 //
 //   * PREFIX: the 32 tokens are 32 rows of a group, the pages a part of its
-//     prefix ("piece"); the CTA leaves (m, l, O) per (row, head) for the decode
+//     prefix ("piece"); the CTA leaves (m, l, O) per (row, head) for the merge
 //     kernel to fold in.  The pieces' length is the shortest that keeps their
 //     number within piece_target (two CTAs per SM), so a few long prefixes and
 //     many short ones both fill the GPU once; every CTA works this out from the
@@ -35,7 +35,7 @@ namespace {
 
 constexpr int kRows = kTileRows * kGroup;          // 128 MMA rows
 constexpr int kChunk = kChunkPages * kPage;        // 64 keys
-constexpr int kStages = 5;
+constexpr int kStages = 4;
 constexpr int kKvBytes = kChunkPages * kTileBytes;  // 8 KiB of K (or of V) per stage
 constexpr int kChunkBytes = 2 * kKvBytes;
 constexpr int kQBytes = kRows * 128;
@@ -75,7 +75,7 @@ __device__ __forceinline__ int2 group_work(const SpanParams& p, int g) {
 
 // Piece `index` of the prefixes, by one warp; group < 0 past the last.  The
 // first block also leaves every group's first piece and count of pieces per
-// stream for the decode kernel.
+// stream for the merge kernel.
 __device__ __forceinline__ Piece find_piece(const SpanParams& p, int index, int lane, bool publish) {
   auto sum = [](long long v) {
 #pragma unroll
@@ -163,8 +163,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   RowSpan span = {};   // window: from list to logical pages
   const int32_t* table;
   if (PREFIX) {
-    // The decode kernel may take the SMs that run out of pieces.
+    // Launched beside the decode kernel (a programmatic dependent launch that
+    // needs nothing of it).  The merge kernel waits for this grid alone, so one
+    // block of it, which has a piece only when there are as many as fit, waits
+    // for the decode kernel.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (!groups_in_order(p)) return;  // the decode kernel reports it
     Piece* shared_piece = reinterpret_cast<Piece*>(smem + kOffPlan);
     if (warp == 0) {
@@ -618,8 +622,17 @@ cudaError_t launch_tiles(const SpanParams& p, long long pool_rows, dim3 grid, cu
   if (!pool_tensor_map(p.k_pool, pool_rows, p.kv_heads, &k_map) ||
       !pool_tensor_map(p.v_pool, pool_rows, p.kv_heads, &v_map))
     return cudaErrorInvalidValue;
-  span_tiles_kernel<PREFIX><<<grid, kThreads, kSmem, stream>>>(p, k_map, v_map);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PREFIX ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, span_tiles_kernel<PREFIX>, p, k_map, v_map);
 }
 
 }  // namespace

@@ -1,6 +1,6 @@
 // Merging the online-softmax states of the consumer warps ("ways") that share
-// a KV head: KVH heads on 16 consumer warps leave W = 16 / KVH ways per head,
-// each over pages of its own.
+// a KV head: KVH heads on 16 consumer warps leave W = 16 / KVH ways per head
+// (on 8 warps, 8 / KVH), each over pages of its own.
 #pragma once
 
 #include "tvp_tile.cuh"
@@ -36,12 +36,12 @@ __device__ __forceinline__ void merge_state(HeadState& a, const float* b) {
 // so that a warp's stores and loads are conflict-free.  Barrier ids: 1 + h for
 // the levels (participants: the ways still in the tree), 1 + KVH + h for the
 // entry, which all W ways pass, so that no way of the next piece writes a slot
-// that way 0 is still reading.  With two ways (KVH = 8) the one level has the
+// that way 0 is still reading.  With two ways the one level has the
 // entry's participants, and both use 1 + h.
-template <int KVH>
+template <int KVH, int W = 16 / KVH>
 __device__ __forceinline__ void merge_ways(HeadState& st, float* scratch, int way, int h,
                                            int lane) {
-  constexpr int W = 16 / KVH;
+  if (W == 1) return;
   named_barrier_sync(W == 2 ? 1 + h : 1 + KVH + h, W * 32);
 #pragma unroll
   for (int d = W / 2; d >= 1; d >>= 1) {
