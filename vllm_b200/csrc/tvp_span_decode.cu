@@ -432,6 +432,11 @@ cudaError_t launch(const SpanParams& p, const CUtensorMap& k_map, const CUtensor
     e = cudaFuncSetAttribute(span_decode_kernel<KVH, SHARED>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)Shape<KVH, SHARED>::kSmem);
+    // The tile kernel's CTAs find their shared memory beside this one's.
+    if (e == cudaSuccess && SHARED)
+      e = cudaFuncSetAttribute(span_decode_kernel<KVH, SHARED>,
+                               cudaFuncAttributePreferredSharedMemoryCarveout,
+                               cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }

@@ -615,6 +615,10 @@ cudaError_t launch_tiles(const SpanParams& p, long long pool_rows, dim3 grid, cu
       return cudaErrorInvalidConfiguration;
     e = cudaFuncSetAttribute(span_tiles_kernel<PREFIX>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)kSmem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(span_tiles_kernel<PREFIX>,
+                               cudaFuncAttributePreferredSharedMemoryCarveout,
+                               cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
