@@ -60,19 +60,6 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
-// Whether the phase with `parity` has completed, without waiting.
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
 // Nanoseconds since `start` by %globaltimer, as a signed difference: a timer
 // that steps back (it is re-synchronised) reads as no time passed instead of
 // wrapping to a huge unsigned interval and ending a wait at once.
@@ -90,6 +77,18 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity)
       if (mbar_try_wait(bar, parity)) return true;
     if (elapsed_ns(start) > (long long)kWaitLimitNs) return false;
   }
+}
+
+// mbar_wait_bounded that sleeps `ns` between its tests: a wait that polls takes
+// issue slots from the warps of its SM sub-partition that have work.
+__device__ __forceinline__ bool mbar_wait_sleeping(uint32_t bar, uint32_t parity, unsigned ns) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long start = global_timer_ns();
+  do {
+    __nanosleep(ns);
+    if (mbar_try_wait(bar, parity)) return true;
+  } while (elapsed_ns(start) <= (long long)kWaitLimitNs);
+  return false;
 }
 
 // Bounded wait until round `round` of a pipeline stage has been issued.  The

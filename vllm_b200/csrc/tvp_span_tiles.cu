@@ -11,11 +11,11 @@
 //   * window: the tokens are a tile of a sequence's queries, the pages the ones
 //     that some query of the tile sees; the CTA writes the output rows.
 //
-// Keys go in chunks of 4 pages (64 keys): warp 0 streams K and V boxes (TMA)
-// into a ring, one thread of warp 1 issues S = Q K^T and O += P V, two softmax
-// sides of four warps (one thread per row) take the chunks in turn, each with
-// its own P and O in Tensor Memory and its own running maximum and sum; they
-// merge at the end.  Unlike K3's, scores stay FP32, and P is written to Tensor
+// Keys go in chunks of 4 pages (64 keys): warps 0 and 3 stream K and V boxes
+// (TMA) into a ring, warp 1 issues S = Q K^T, warp 2 O += P V, two softmax sides
+// of four warps (one thread per row) take the chunks in turn, each with its own
+// P and O in Tensor Memory and its own running maximum and sum; they merge at
+// the end.  Unlike K3's, scores stay FP32, and P is written to Tensor
 // Memory (two BF16 per column) and is the MMA's A operand there: shared memory
 // carries no P, whose write and reads took half of its bandwidth (per 64-key
 // chunk and tile 16 KB written and 16 KB read, next to 24 KB for S, 8 KB for V
@@ -23,9 +23,9 @@
 // A side takes a chunk's scores into registers at once, so one S of 64 columns
 // serves both, and S(c + 2) is formed while chunk c is still in its
 // exponentials.  (With an S per side that P overwrote, S(c + 2) had to wait for
-// P V(c): a side idled 1000 of 3200 cycles per chunk.)  The MMA thread issues
-// S(0), then per chunk c: [wait: S(c) read] S(c + 1), [wait: P(c - 1) written]
-// P V(c - 1); a side waits for P V(c - 2) before it rescales its O or writes P(c).
+// P V(c): a side idled 1000 of 3200 cycles per chunk.)  S(c + 1) follows when
+// S(c) was read, P V(c) when P(c) was written; a side waits for P V(c - 2) before
+// it rescales its O or writes P(c).
 #include "tvp_span.cuh"
 #include "tvp_tile.cuh"
 #include "tvp_umma.cuh"
@@ -45,12 +45,14 @@ constexpr uint32_t kTmemCols = 256;
 constexpr uint32_t kColP = 64, kColO = 128;
 constexpr int kLowRegs = 32;    // warps 0-3
 constexpr int kHighRegs = 104;  // the softmax warps
+constexpr unsigned kProducerNs = 200, kMmaNs = 40;  // sleeps of the waiting warps
 constexpr int kMinChunks = 2;   // a piece of a prefix is no shorter than this
 
 constexpr int kOffStages = kQBytes;
 constexpr int kOffBars = kOffStages + kStages * kChunkBytes;
-// q_full, o_full, drain, (unused), then by side: S formed, S read, P written, P V
+// q_full, o_full, drain[2], then by side: S formed, S read, P written, P V
 // done; kv_full[stages], kv_empty[stages]
+constexpr int kBarDrain = 2;
 constexpr int kBarSFull = 4;
 constexpr int kBarSRead = 6;
 constexpr int kBarPFull = 8;
@@ -212,14 +214,14 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
   auto bar = [&](int i) { return smem_addr(&bars[i]); };
-  const uint32_t q_full = bar(0), o_full = bar(1), drain = bar(2);
+  const uint32_t q_full = bar(0), o_full = bar(1);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int quarters = (count * kGroup + 31) / 32;  // row quarters with a real row
   if (threadIdx.x == 0) {
     mbar_init(q_full, 4);
     mbar_init(o_full, 1);
-    mbar_init(drain, 1);
+    mbar_init(bar(kBarDrain), 1);
+    mbar_init(bar(kBarDrain + 1), 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar(kBarSFull + b), 1);
       mbar_init(bar(kBarSRead + b), quarters);
@@ -227,10 +229,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(bar(kBarPvDone + b), 1);
     }
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(bar(kBarKvFull + i), 1);
+      mbar_init(bar(kBarKvFull + i), 2);  // K and V
       mbar_init(bar(kBarKvEmpty + i), 1);
     }
-    *abort_flag = 0;
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -241,138 +242,140 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  // Threads that meet before Tensor Memory is released: warp 1 and both sides.
-  constexpr int kEndThreads = 32 + 8 * 32;
+  // Threads that meet before Tensor Memory is released: warps 1, 2 and both sides.
+  constexpr int kEndThreads = 2 * 32 + 8 * 32;
 
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLowRegs));
-    if (warp >= 2) return;  // the rest of this warpgroup only hands its registers over
-  }
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLowRegs));
 
-  if (warp == 0) {
-    // ------------------------------ producer ------------------------------
-    if (lane == 0) {
-      prefetch_tensor_map(&k_map);
-      prefetch_tensor_map(&v_map);
-    }
-    // lanes 0-3: K box of page slot `lane`, lanes 4-7: V box of slot lane - 4;
-    // the next chunk's page ids are loaded one chunk ahead.
-    auto page_id = [&](int c) {
+  if (warp == 0 || warp == 3) {
+    // ------------------------------ producers -----------------------------
+    // Warp 0 streams K, warp 3 V: a box takes some 100 cycles to issue, and the
+    // eight of a chunk by one warp took longer than its exponentials.
+    const CUtensorMap* map = warp == 0 ? &k_map : &v_map;
+    const uint32_t dst0 = sbase + kOffStages + (warp == 0 ? 0 : kKvBytes);
+    if (lane == 0) prefetch_tensor_map(map);
+    const int chunks = __shfl_sync(0xffffffffu, n_chunks, 0);
+    const int x = __shfl_sync(0xffffffffu, g, 0) * kHeadDim;
+    // lane i: the row of the pool that page slot i of a chunk starts at, -16 for a
+    // slot past the last page or a bad id (a box wholly outside the pool arrives as
+    // zeros); loaded one chunk ahead.
+    auto page_row = [&](int c) {
       const int v = v_begin + c * kChunkPages + (lane & 3);
-      return lane < 8 && v < v_end ? __ldg(table + span.logical(v)) : -1;
+      if (v >= v_end) return -kPage;
+      const int phys = __ldg(table + span.logical(v));
+      if (phys >= 0 && phys < p.num_pages) return (int)(p.layer_row_base + (long long)phys * kPage);
+      if (warp == 0 && lane < kChunkPages) record_error(p.err, TVP_DEVERR_BAD_PAGE);
+      return -kPage;
     };
-    int issued = 0;
-    int next = page_id(0);
-    for (int c = 0; c < n_chunks; ++c) {
-      const int st = c % kStages;
-      const int phys = next;
-      if (c + 1 < n_chunks) next = page_id(c + 1);
-      if (c >= kStages) {
-        int timed_out = 0;
-        if (lane == 0) timed_out = !mbar_wait_bounded(bar(kBarKvEmpty + st), ((c / kStages) - 1) & 1);
-        if (__shfl_sync(0xffffffffu, timed_out, 0)) {
-          if (lane == 0) {
-            *abort_flag = 1;
-            record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_EMPTY);
-          }
-          break;
-        }
+    int issued = 0, stage = 0, parity = 1;  // of the round before
+    int next = page_row(0);
+    for (int c = 0; c < chunks; ++c) {
+      const int rows = next;
+      if (c + 1 < chunks) next = page_row(c + 1);
+      if (c >= kStages &&
+          !__all_sync(0xffffffffu, mbar_wait_sleeping(bar(kBarKvEmpty + stage), parity, kProducerNs))) {
+        if (lane == 0) record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_EMPTY);
+        break;
       }
-      const bool real = lane < 8 && v_begin + c * kChunkPages + (lane & 3) < v_end;
-      const bool ok = real && phys >= 0 && phys < p.num_pages;
-      if (real && !ok && lane < 4) record_error(p.err, TVP_DEVERR_BAD_PAGE);
-      if (lane == 0) mbar_arrive_expect_tx(bar(kBarKvFull + st), kChunkBytes);
+      int y[kChunkPages];
+#pragma unroll
+      for (int i = 0; i < kChunkPages; ++i) y[i] = __shfl_sync(0xffffffffu, rows, i);
+      if (elect_one()) {
+        const uint32_t full = bar(kBarKvFull + stage);
+        mbar_arrive_expect_tx(full, kKvBytes);
+#pragma unroll
+        for (int i = 0; i < kChunkPages; ++i)
+          tma_load_2d(dst0 + stage * kChunkBytes + i * kTileBytes, map, x, y[i], full);
+      }
       __syncwarp();
-      if (lane < 8) {
-        const uint32_t dst = sbase + kOffStages + st * kChunkBytes + (lane < 4 ? 0 : kKvBytes) +
-                             (lane & 3) * kTileBytes;
-        // A box wholly outside the pool (rows -16 .. -1) arrives as zeros.
-        const int y = ok ? (int)(p.layer_row_base + (long long)phys * kPage) : -kPage;
-        tma_load_2d(dst, lane < 4 ? &k_map : &v_map, g * kHeadDim, y, bar(kBarKvFull + st));
-      }
       issued = c + 1;
+      if (++stage == kStages) {
+        stage = 0;
+        parity ^= 1;
+      }
     }
     drain_issued_stages<kStages>(bars + kBarKvFull, issued, lane, p.err);
     return;
   }
 
-  if (warp == 1) {
-    // ------------------------------ MMA issuer ----------------------------
-    // The whole warp waits and works out the operands, one lane issues.
+  if (warp <= 2) {
+    // ----------------------------- MMA issuers ----------------------------
+    // Warp 1 issues S(c), warp 2 P V(c): a wait takes some 300 cycles even where
+    // nothing is to be waited for, and one warp after three of them per chunk held
+    // every chunk up by 1550 cycles.  The whole warp waits and works out the
+    // operands, one lane issues.
     constexpr uint32_t kIdS = umma_idesc_bf16_f32(kRows, kChunk, false, false);
     constexpr uint32_t kIdO = umma_idesc_bf16_f32(kRows, kHeadDim, false, true);
     const uint32_t cols = __shfl_sync(0xffffffffu, tmem, 0);
     const int chunks = __shfl_sync(0xffffffffu, n_chunks, 0);
-    // Descriptors of Q and of stage 0's K and V; a byte offset adds offset / 16.
-    const uint64_t q_desc = umma_desc_sw128(sbase, 16, 1024);
-    const uint64_t k_desc = umma_desc_sw128(sbase + kOffStages, 16, 1024);
-    const uint64_t v_desc = umma_desc_sw128(sbase + kOffStages + kKvBytes, 0, 1024);
     bool ok = true;
     auto wait = [&](uint32_t b, uint32_t parity) {
-      if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(b, parity))) {
+      if (ok && !__all_sync(0xffffffffu, mbar_wait_sleeping(b, parity, kMmaNs))) {
         if (lane == 0) record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_FULL);
         ok = false;
       }
       return ok;
     };
-    // S(c) = Q K(c)^T, 16 channels per MMA, for side c % 2.
-    int s_stage = 0, s_parity = 0;  // of the next chunk of S
-    auto issue_s = [&](int c) {
-      if (!wait(bar(kBarKvFull + s_stage), s_parity)) return;
-      tc_fence_after_sync();
-      const uint64_t k = k_desc + (uint32_t)(s_stage * (kChunkBytes >> 4));
-      if (elect_one()) {
-#pragma unroll
-        for (int i = 0; i < kHeadDim / 16; ++i)
-          umma_bf16(cols, q_desc + 2 * i, k + 2 * i, kIdS, i > 0);
-        umma_commit(bar(kBarSFull + (c & 1)));
-      }
-      __syncwarp();
-      if (++s_stage == kStages) {
-        s_stage = 0;
-        s_parity ^= 1;
-      }
-    };
-    wait(q_full, 0);
-    issue_s(0);
     int stage = 0;
-    for (int c = 0; ok && c <= chunks; ++c) {
-      if (c + 1 < chunks) {  // S(c) is in the registers of its side
-        if (!wait(bar(kBarSRead + (c & 1)), (c >> 1) & 1)) break;
-        issue_s(c + 1);
-      }
-      if (c == 0) continue;
-      // O_s += P(d) V(d) for d = c - 1 and its side s, 16 keys (one page of V, 8
-      // columns of P) per MMA; the first chunk of each side overwrites O.
-      const int d = c - 1, side = d & 1;
-      if (!wait(bar(kBarPFull + side), (d >> 1) & 1)) break;
-      tc_fence_after_sync();
-      const uint64_t v = v_desc + (uint32_t)(stage * (kChunkBytes >> 4));
-      if (elect_one()) {
+    if (warp == 1) {
+      // S(c) = Q K(c)^T for side c % 2, 16 channels per MMA, once S(c - 1) is in the
+      // registers of its side.  Descriptors: a byte offset adds offset / 16.
+      const uint64_t q_desc = umma_desc_sw128(sbase, 16, 1024);
+      const uint64_t k_desc = umma_desc_sw128(sbase + kOffStages, 16, 1024);
+      int parity = 0;
+      wait(q_full, 0);
+      for (int c = 0; ok && c < chunks; ++c) {
+        if (!wait(bar(kBarKvFull + stage), parity)) break;
+        if (c > 0 && !wait(bar(kBarSRead + ((c - 1) & 1)), ((c - 1) >> 1) & 1)) break;
+        tc_fence_after_sync();
+        const uint64_t k = k_desc + (uint32_t)(stage * (kChunkBytes >> 4));
+        if (elect_one()) {
 #pragma unroll
-        for (int i = 0; i < kChunkPages; ++i)
-          umma_bf16_ts(cols + kColO + 64 * side, cols + kColP + 32 * side + 8 * i,
-                       v + (uint32_t)(i * (kTileBytes >> 4)), kIdO, (d >= 2 || i > 0));
-        umma_commit(bar(kBarPvDone + side));
-        umma_commit(bar(kBarKvEmpty + stage));
+          for (int i = 0; i < kHeadDim / 16; ++i)
+            umma_bf16(cols, q_desc + 2 * i, k + 2 * i, kIdS, i > 0);
+          umma_commit(bar(kBarSFull + (c & 1)));
+        }
+        __syncwarp();
+        if (++stage == kStages) {
+          stage = 0;
+          parity ^= 1;
+        }
       }
-      __syncwarp();
-      if (++stage == kStages) stage = 0;
+    } else {
+      // O_s += P(c) V(c) for c's side s, 16 keys (one page of V, 8 columns of P) per
+      // MMA; the first chunk of each side overwrites O.  V(c) is there: P(c) comes
+      // of S(c), which waited for the chunk.
+      const uint64_t v_desc = umma_desc_sw128(sbase + kOffStages + kKvBytes, 0, 1024);
+      for (int c = 0; ok && c < chunks; ++c) {
+        const int side = c & 1;
+        if (!wait(bar(kBarPFull + side), (c >> 1) & 1)) break;
+        tc_fence_after_sync();
+        const uint64_t v = v_desc + (uint32_t)(stage * (kChunkBytes >> 4));
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < kChunkPages; ++i)
+            umma_bf16_ts(cols + kColO + 64 * side, cols + kColP + 32 * side + 8 * i,
+                         v + (uint32_t)(i * (kTileBytes >> 4)), kIdO, (c >= 2 || i > 0));
+          umma_commit(bar(kBarPvDone + side));
+          umma_commit(bar(kBarKvEmpty + stage));
+        }
+        __syncwarp();
+        if (++stage == kStages) stage = 0;
+      }
+      if (ok && elect_one()) umma_commit(o_full);
     }
-    if (!ok && lane == 0) *abort_flag = 1;
-    if (elect_one()) {
-      if (ok) umma_commit(o_full);
-      // Every MMA issued has completed before Tensor Memory is released.
-      umma_commit(drain);
-    }
+    // Every MMA issued has completed before Tensor Memory is released.
+    if (elect_one()) umma_commit(bar(kBarDrain + warp - 1));
     __syncwarp();
-    if (!__all_sync(0xffffffffu, mbar_wait_bounded(drain, 0)) && lane == 0)
+    if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar(kBarDrain + warp - 1), 0)) && lane == 0)
       record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_DRAIN);
     __syncwarp();
     tc_fence_before_sync();
     named_barrier_sync(1, kEndThreads);
-    tc_fence_after_sync();
-    tmem_dealloc(tmem, kTmemCols);
+    if (warp == 1) {
+      tc_fence_after_sync();
+      tmem_dealloc(tmem, kTmemCols);
+    }
     return;
   }
 
@@ -420,28 +423,18 @@ __global__ void __launch_bounds__(kThreads, 2)
     whole1 = (pos0 + 1) / kPage - span.skip;
     sinks_whole = min(span.head, p.sinks / kPage);
   }
-  // A wait of the whole warp, after a test of the barrier made earlier (a wait
-  // costs some 250 cycles of latency even when there is nothing to wait for);
-  // false when it ran out.
-  auto warp_wait = [&](uint32_t b, uint32_t parity, bool tested) {
-    if (__all_sync(0xffffffffu, tested)) return true;
-    if (__all_sync(0xffffffffu, mbar_wait_bounded(b, parity))) return true;
-    if (lane == 0 && !*abort_flag) {
-      *abort_flag = 1;
-      record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_FULL);
-    }
-    return false;
+  // A wait of the whole warp; false when it ran out.
+  auto warp_wait = [&](uint32_t b, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(b, parity)) != 0;
   };
   uint32_t parity = 0;
-  bool s_formed = false, pv_done = false;
   for (int c = side; active && c < n_chunks; c += 2) {
-    ok = warp_wait(bar(kBarSFull + side), parity, s_formed);
+    ok = warp_wait(bar(kBarSFull + side), parity);
     if (!ok) break;
     tc_fence_after_sync();
     uint32_t sr[2][32];
     tmem_ld32(tmem + lane_base, sr[0]);
     tmem_ld32(tmem + 32 + lane_base, sr[1]);
-    if (c >= 2) pv_done = mbar_test(bar(kBarPvDone + side), parity ^ 1u);
     tmem_wait_ld();
     tc_fence_before_sync();
     __syncwarp();
@@ -473,22 +466,23 @@ __global__ void __launch_bounds__(kThreads, 2)
         mx[e] = max3(mx[e], __uint_as_float(sr[0][j + e]), __uint_as_float(sr[1][j + e]));
     }
     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c_log2;
-    // Lazy running max: rescale only when a score beats the side's max by more
-    // than kLazyMargin (probabilities stay below 2^kLazyMargin).
-    float alpha = 1.f;
-    if (top > m + kLazyMargin) {
-      alpha = m == -INFINITY ? 0.f : fast_exp2(m - top);
-      m = top;
-    }
     if (c >= 2) {  // P V(c - 2) is the last MMA into this side's O and out of its P
-      ok = warp_wait(bar(kBarPvDone + side), parity ^ 1u, pv_done);
+      ok = warp_wait(bar(kBarPvDone + side), parity ^ 1u);
       if (!ok) break;
       tc_fence_after_sync();
     }
     parity ^= 1u;
-    if (c >= 2 && __any_sync(0xffffffffu, alpha != 1.f)) {
+    // Lazy running max: rescale only when a score beats the side's max by more
+    // than kLazyMargin (probabilities stay below 2^kLazyMargin).
+    if (__any_sync(0xffffffffu, top > m + kLazyMargin)) {
+      float alpha = 1.f;
+      if (top > m + kLazyMargin) {
+        alpha = m == -INFINITY ? 0.f : fast_exp2(m - top);
+        m = top;
+      }
+      l *= alpha;
 #pragma unroll 1
-      for (int part = 0; part < 4; ++part) {
+      for (int part = 0; c >= 2 && part < 4; ++part) {
         const uint32_t taddr = tmem + kColO + 64 * side + 16 * part + lane_base;
         uint32_t o[16];
         tmem_ld16(taddr, o);
@@ -520,11 +514,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       tmem_st16(tmem + kColP + 32 * side + 16 * half + lane_base, w);
     }
-    s_formed = mbar_test(bar(kBarSFull + side), parity);  // of this side's next chunk
     tmem_wait_st();
     float la, lb;
     f2_unpack(f2_add(f2_add(ls2[0], ls2[1]), f2_add(ls2[2], ls2[3])), la, lb);
-    l = l * alpha + (la + lb);
+    l += la + lb;
     // Tokens that no row of the tile sees may hold anything: zero them in the V
     // tile before P V reads it (P is 0 there, but 0 x NaN is not).
     if (!PREFIX && !whole && quarter == 0) {
@@ -543,7 +536,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(kBarPFull + side));
   }
-  const bool fin = active && ok && warp_wait(o_full, 0, false);
+  const bool fin = active && ok && warp_wait(o_full, 0);
+  if (active && !fin && lane == 0)
+    record_error(p.err, TVP_DEVERR_TIMEOUT | TVP_DEVERR_WAIT_FULL);
   // Merge the two sides per row: side 1 hands its (max, normaliser) to side 0
   // through the Q tile, whose last reader (an S MMA) completed before o_full.
   float* xchg = reinterpret_cast<float*>(smem);
