@@ -400,17 +400,18 @@ __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const Sp
   const int t = g >= 0 ? s - __ldg(p.group_rows + g) : 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   Fold f;
-  if (g >= 0) {
-    const int2 at = __ldcg(p.group_pieces + g);
-    const float* base = p.pieces + ((size_t)(at.x + ((t / kTileRows) * KVH + h) * at.y) * kTileRows +
+  // The prefix's pieces, then the row's own; both counts in one round trip.
+  const int2 at = g >= 0 ? __ldcg(p.group_pieces + g) : make_int2(0, 0);
+  const int2 r = span.pages > 0 ? __ldcg(p.row_ranges + s) : make_int2(0, -1);
+  const float* shared = p.pieces + ((size_t)(at.x + ((t / kTileRows) * KVH + h) * at.y) * kTileRows +
                                     t % kTileRows) * kPartialFloats;
-    f.add_all(at.y, [&](int i) { return base + (size_t)i * kPieceFloats; }, lane);
-  }
-  if (span.pages > 0) {
-    const int2 r = __ldcg(p.row_ranges + s);
-    const float* base = p.partials + ((size_t)(s + r.x) * KVH + h) * kPartialFloats;
-    f.add_all(r.y - r.x + 1, [&](int i) { return base + (size_t)i * KVH * kPartialFloats; }, lane);
-  }
+  const float* own = p.partials + ((size_t)(s + r.x) * KVH + h) * kPartialFloats;
+  f.add_all(at.y + r.y - r.x + 1,
+            [&](int i) {
+              return i < at.y ? shared + (size_t)i * kPieceFloats
+                              : own + (size_t)(i - at.y) * KVH * kPartialFloats;
+            },
+            lane);
   f.write(p.out + ((size_t)s * KVH + h) * kGroup * kHeadDim, lane);
 }
 
