@@ -156,6 +156,24 @@ def test_prefill_chunks(kv_heads, window, sinks):
     S.check(got, case, f"heads {kv_heads} window {window} sinks {sinks}")
 
 
+@pytest.mark.parametrize("window", [1, 3, 20, 64])
+@pytest.mark.parametrize("sinks", [64, 100, 500, 1 << 30])
+def test_prefill_sinks_that_reach_past_the_queries(window, sinks):
+    """Sinks beyond a tile's own positions, whose chunks are not visible as a whole."""
+    case = S.SpanCase(88, [52, 113, 700, 63], kv_heads=2, window=window, sinks=sinks, q_counts=[3, 40, 300, 1])
+    got, err = run_prefill(case)
+    assert err == 0
+    S.check(got, case, f"window {window} sinks {sinks}")
+
+
+@pytest.mark.parametrize("sinks", [100, 1 << 30])
+def test_decode_sinks_past_the_window(sinks):
+    case = S.SpanCase(89, [52, 113, 700, 63], window=1, sinks=sinks)
+    got, err = run_decode(case)
+    assert err == 0
+    S.check(got, case)
+
+
 @pytest.mark.parametrize("window,sinks", [(200, 4), (513, 0), (129, 130)])
 def test_prefill_longer_prompts(window, sinks):
     case = S.SpanCase(90, [1500, 900], kv_heads=2, window=window, sinks=sinks, q_counts=[1500, 77], num_layers=2,

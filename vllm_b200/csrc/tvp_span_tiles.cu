@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     whole0 = max(span.head, first - span.skip);
     if (span.skip == 0) whole0 = first;
     whole1 = (pos0 + 1) / kPage - span.skip;
-    sinks_whole = min(span.head, p.sinks / kPage);
+    sinks_whole = min(min(span.head, p.sinks / kPage), (pos0 + 1) / kPage);  // none in the future
   }
   // A wait of the whole warp; false when it ran out.
   auto warp_wait = [&](uint32_t b, uint32_t parity) {
