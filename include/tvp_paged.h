@@ -425,10 +425,9 @@ size_t tvp_span_workspace_bytes(int batch, int groups, int kv_heads, int num_cta
  * sinks >= 0; a row with L <= 0 gets zeros (negative: TVP_DEVERR_BAD_LENGTH).
  * Pages without a visible token are not read: their table entries may be
  * anything (-1 once the page was given back), and hidden tokens of pages that
- * are read may hold NaN.  No plan is needed: d_seq_lens is read by the kernel.
- * As tvp_paged_decode_attention, the launch is a programmatic dependent one:
- * a kernel that releases its dependents early must not write d_seq_lens or the
- * block tables when it runs right before this call.
+ * are read may hold NaN.  No plan is needed: d_seq_lens is read by the kernel,
+ * after the kernel before it on the stream has finished (the launch is a
+ * programmatic dependent one).
  */
 int tvp_paged_window_decode_attention(const tvp_bf16* q, const tvp_bf16* k_pool,
                                       const tvp_bf16* v_pool, int num_pages, int num_layers,

@@ -169,3 +169,37 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         assert int(err.item()) == 0
         S.check(host_bf16(out), case)
+
+
+def test_many_small_groups():
+    """More groups than a warp has lanes, some without a prefix or without rows."""
+    rng = np.random.default_rng(6)
+    groups = [(int(n), int(p)) for n, p in zip(rng.integers(0, 5, 150), rng.integers(0, 6, 150))]
+    case = S.SpanCase(34, rows(rng, groups, 40), groups=groups, kv_heads=2)
+    got, err = run(case)
+    assert err == 0
+    S.check(got, case)
+
+
+def test_two_groups_on_the_same_pages():
+    """A prefix that two groups name."""
+    case = S.SpanCase(35, [70, 64, 90, 100], groups=[(2, 3), (2, 3)])
+    case.prefix_tables[1] = case.prefix_tables[0]
+    case.full[2:, :3] = case.prefix_tables[0, :3]
+    got, err = run(case)
+    assert err == 0
+    S.check(got, case)
+
+
+def test_one_workspace_for_both_decode_forms():
+    """Calls of both forms and of different sizes in turn on one workspace."""
+    import test_window_attention_gpu as T
+    groups = [(9, 21), (36, 13)]
+    shared = S.SpanCase(36, rows(np.random.default_rng(7), groups, 300), groups=groups)
+    windows = S.SpanCase(37, [700, 33, 1, 3000, 250, 17, 1600, 0, 16], window=900, sinks=20)
+    ws = ops.SpanWorkspace(45, "cuda", max_groups=2)
+    for _ in range(3):
+        for case, call in ((shared, run), (windows, T.run_decode)):
+            got, err = call(case, workspace=ws)
+            assert err == 0
+            S.check(got, case)

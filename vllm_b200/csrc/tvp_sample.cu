@@ -1,8 +1,9 @@
 // K9 — one token per row of logits from given random numbers.
 //
-// A cluster of 8 CTAs takes a row: each keeps its eighth of the logits in
-// shared memory, so the row is read once from HBM however many passes the
-// filters take, and a single row streams through 8 SMs.
+// A cluster of CTAs takes a row: 8 that keep the logits in shared memory while
+// there are few rows, so that a row is read once from HBM however many passes
+// the filters take, and 4 or 2 that read them again from L2 when there are many
+// (kStreamRows).
 //
 // Weights.  w_i = exp((x_i - max) / T) is held as an integer of 2^-44 of the
 // largest weight, so sums are exact in any order (atomics included) and every
@@ -15,13 +16,21 @@
 // Filters.  top-k and top-p cut the row at a place in its falling order (value,
 // then index).  A histogram of the distance from the maximum, 2048 buckets over
 // the distances that still have weight, finds the bucket of the cut; each CTA
-// bins its eighth, CTA r adds up buckets [256 r, 256 r + 256) of all eight
-// through distributed shared memory.  When few enough logits lie at or above
-// that bucket (a usual nucleus), CTA 0 gathers them, cuts and draws, all by
-// comparing each with each; 4 cluster barriers in all.  Otherwise only the cut's
-// own bucket is gathered (or, when it holds many, resolved by radix digits and a
-// count of equal logits by index), and the draw goes by sums: per CTA, per warp,
-// then within the warp's segment in index order.
+// bins its part, CTA r adds up its share of the buckets of all of them through
+// distributed shared memory.  When few enough logits lie at or above that bucket
+// (a usual nucleus), CTA 0 gathers them, cuts and draws, all by comparing each
+// with each.  Otherwise only the cut's own bucket is gathered (or, when it holds
+// many, resolved by radix digits and a count of equal logits by index), and the
+// draw goes by sums: per CTA, per 128 neighbouring logits, then by one warp over
+// the 128 at the point.  For a small top-k the histogram is one of the largest
+// logits of every 32, which costs no pass over the row.
+//
+// What bounds it, at rows of 128256 logits: one row 8.5 us without filters, 11
+// with top-k 50, 27 with top-p 0.9 (launch, cluster barriers of about 1 us each,
+// and passes of one row over 8 SMs); 256 rows without filters 67 us (131 MB: 2.0
+// TB/s; the weights' FP64 arithmetic takes 50 of them), with top-k 50 47 us (2.8
+// TB/s, two passes of which one is from L2), with top-p 0.9 202 us (a weight
+// into a shared-memory histogram, two 32-bit atomics, for each logit with one).
 #include <cfloat>
 #include <climits>
 
@@ -80,7 +89,7 @@ struct alignas(16) Shared {
   u64 amount[CL];  // by rank: a sum that the step at hand exchanges
   int fills[2][CL];  // in turn: one gather() may follow another at once
   u64 ties[CL];
-  u64 seg[CL > 1 ? kSegment : 1];  // this CTA's segment of the cluster's histogram
+  u64 seg[kSegment];  // this CTA's segment of the cluster's histogram
   u64 sub[kBlocks];                // every 32 buckets of the whole histogram
   u64 warp[kWarps];
   float warp_most[kWarps], warp_least[kWarps];
@@ -182,15 +191,10 @@ struct Sampler {
   int turn;
 
   // The CTAs of a row: barrier, and another one's shared memory.
-  __device__ static void sync() {
-    if (CL > 1)
-      cg::this_cluster().sync();
-    else
-      __syncthreads();
-  }
+  __device__ static void sync() { cg::this_cluster().sync(); }
   template <typename V>
   __device__ static V* of_rank(V* place, int r) {
-    return CL > 1 ? cg::this_cluster().map_shared_rank(place, r) : place;
+    return cg::this_cluster().map_shared_rank(place, r);
   }
 
   // A thread's batch `it` is the kQuads quads of logits (it kQuads + e) kThreads +
@@ -329,34 +333,26 @@ struct Sampler {
       });
     }
     sync();
-    if (CL > 1) {
-      // This CTA's segment over all, and the sum of each warp's 32 buckets to
-      // every CTA.
-      for (int i = tid; i < kSegment; i += kThreads) {
-        const int b = rank * kSegment + i;
-        u64 as[CL], a = 0;
+    // This CTA's segment over all, and the sum of each warp's 32 buckets to
+    // every CTA.
+    for (int i = tid; i < kSegment; i += kThreads) {
+      const int b = rank * kSegment + i;
+      u64 as[CL], a = 0;
 #pragma unroll
-        for (int r = 0; r < CL; ++r) as[r] = MASS ? of_rank(hist, r)[b] : of_rank(counts, r)[b];
+      for (int r = 0; r < CL; ++r) as[r] = MASS ? of_rank(hist, r)[b] : of_rank(counts, r)[b];
 #pragma unroll
-        for (int r = 0; r < CL; ++r) a += as[r];
-        s.seg[i] = a;
-        a = warp_sum(a);
-        if (lane < CL) of_rank(s.sub, lane)[b / 32] = a;
-      }
-    } else {
-      for (int block = warp; block < kBlocks; block += kWarps) {
-        const int i = block * 32 + lane;
-        const u64 a = warp_sum(MASS ? hist[i] : counts[i]);
-        if (lane == 0) s.sub[block] = a;
-      }
+      for (int r = 0; r < CL; ++r) a += as[r];
+      s.seg[i] = a;
+      a = warp_sum(a);
+      if (lane < CL) of_rank(s.sub, lane)[b / 32] = a;
     }
     sync();
     // One warp finds the 32 buckets, then the bucket.
-    if (warp == 0) find_border<MASS>(want_of);
+    if (warp == 0) find_border(want_of);
     __syncthreads();
     return s.border;
   }
-  template <bool MASS, typename Want>
+  template <typename Want>
   __device__ __forceinline__ void find_border(Want want_of) {
     Border out;
     const u64 s0 = s.sub[2 * lane], s1 = s.sub[2 * lane + 1];
@@ -374,14 +370,8 @@ struct Sampler {
     const bool second = before + s0 < out.want;
     const int block = 2 * src + __shfl_sync(0xffffffffu, (int)second, src);
     const u64 above = __shfl_sync(0xffffffffu, second ? before + s0 : before, src);
-    u64 mine;
-    if (CL > 1) {
-      constexpr int kPer = kSegment / 32;  // blocks of a CTA
-      mine = of_rank(s.seg, block / kPer)[block % kPer * 32 + lane];
-    } else {
-      mine = MASS ? reinterpret_cast<const u64*>(scratch)[block * 32 + lane]
-                  : reinterpret_cast<const uint32_t*>(scratch)[block * 32 + lane];
-    }
+    constexpr int kPer = kSegment / 32;  // blocks of a CTA
+    const u64 mine = of_rank(s.seg, block / kPer)[block % kPer * 32 + lane];
     const u64 upto = above + warp_scan(mine, lane);
     const int hit = __ffs(__ballot_sync(0xffffffffu, upto >= out.want)) - 1;
     out.bin = block * 32 + hit;
@@ -395,7 +385,7 @@ struct Sampler {
   __device__ u64* list() const { return reinterpret_cast<u64*>(scratch) + kList; }
   __device__ u64* weights() const { return reinterpret_cast<u64*>(scratch) + 2 * kList; }
   __device__ int gather(int b0, int b1, int most) {
-    u64* mine = CL == 1 ? list() : reinterpret_cast<u64*>(scratch);
+    u64* mine = reinterpret_cast<u64*>(scratch);
     // A logit of bucket b1 lies above this (the distance is rounded, by 2^-23 of it
     // at most, and so are the product and the quotient).
     const float reach =
@@ -429,7 +419,6 @@ struct Sampler {
       put(v.w, i + 3);
     });
     __syncthreads();
-    if (CL == 1) return s.fill;
     int* fills = s.fills[turn ^= 1];
     share(fills, s.fill);
     int n = 0;
@@ -632,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                   const float* __restrict__ min_p, int32_t* __restrict__ tokens) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Shared<CL> s;
-  const int rank = CL > 1 ? (int)cg::this_cluster().block_rank() : 0, row = blockIdx.x / CL;
+  const int rank = (int)cg::this_cluster().block_rank(), row = blockIdx.x / CL;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int begin = min(rank * slice, vocab), len = min(slice, vocab - begin);
   const float* src = logits + (size_t)row * row_stride + begin;
@@ -696,17 +685,15 @@ __global__ void __launch_bounds__(kThreads, 2)
     top = fmaxf(top, s.warp_most[w]);
     lo = fminf(lo, s.warp_least[w]);
   }
-  if (CL > 1) {
-    if (tid < CL) {
-      Sampler<CL, RES>::of_rank(s.most, tid)[rank] = top;
-      Sampler<CL, RES>::of_rank(s.least, tid)[rank] = lo;
-    }
-    Sampler<CL, RES>::sync();
+  if (tid < CL) {
+    Sampler<CL, RES>::of_rank(s.most, tid)[rank] = top;
+    Sampler<CL, RES>::of_rank(s.least, tid)[rank] = lo;
+  }
+  Sampler<CL, RES>::sync();
 #pragma unroll
-    for (int r = 0; r < CL; ++r) {
-      top = fmaxf(top, s.most[r]);
-      lo = fminf(lo, s.least[r]);
-    }
+  for (int r = 0; r < CL; ++r) {
+    top = fmaxf(top, s.most[r]);
+    lo = fminf(lo, s.least[r]);
   }
   if (top == -INFINITY) {
     if (rank == 0 && tid == 0) tokens[row] = -1;
@@ -896,7 +883,7 @@ cudaError_t launch_sampler(int rows, int vocab, long long row_stride, const floa
                            const float* uniforms, const float* temperature, const int32_t* top_k,
                            const float* top_p, const float* min_p, int32_t* tokens,
                            cudaStream_t stream) {
-  auto slice_of = [](int v) { return CL > 1 ? ((v + CL - 1) / CL + 3) / 4 * 4 : v; };
+  auto slice_of = [](int v) { return ((v + CL - 1) / CL + 3) / 4 * 4; };
   auto smem_of = [](int slice) {
     return kScratchBytes + (size_t)batches_of(slice) * kThreads * 4 + (RES ? (size_t)slice * 4 + 16 : 0);
   };
