@@ -26,7 +26,8 @@ COMMON = [({"q": None}, INVALID), ({"k": None}, INVALID), ({"v": None}, INVALID)
           ({"tables": None}, INVALID), ({"pages": 0}, INVALID), ({"layer": 16}, INVALID), ({"layer": -1}, INVALID),
           ({"stride": 0}, INVALID), ({"scale": float("nan")}, INVALID), ({"scale": float("inf")}, INVALID),
           ({"kvh": 3, "qh": 12}, UNSUPPORTED), ({"kvh": 16, "qh": 64}, UNSUPPORTED), ({"qh": 16}, UNSUPPORTED),
-          ({"pages": 1 << 24}, UNSUPPORTED), ({"k": ODD}, INVALID), ({"out": ODD}, INVALID)]
+          ({"pages": 1 << 24}, UNSUPPORTED), ({"k": ODD}, INVALID), ({"out": ODD}, INVALID),
+          ({"stride": 1 << 27}, UNSUPPORTED)]
 ROWS = [({"lens": None}, INVALID), ({"batch": 0}, INVALID), ({"batch": -1}, INVALID), ({"ctas": -1}, INVALID),
         ({"ctas": 1025}, INVALID), ({"ws": None}, WORKSPACE), ({"wsb": 1 << 10}, WORKSPACE), ({"ws": ODD}, WORKSPACE)]
 WIN = [({"window": 0}, INVALID), ({"window": -5}, INVALID), ({"sinks": -1}, INVALID)]
@@ -47,7 +48,8 @@ def test_window_decode_refuses(native):
 def test_shared_prefix_refuses(native):
     refused(native.tvp_paged_shared_prefix_decode_attention, SHARED, COMMON + ROWS + [
         ({"groups": -1}, INVALID), ({"groups": 65536}, INVALID), ({"ptables": None}, INVALID),
-        ({"ppages": None}, INVALID), ({"rows": None}, INVALID), ({"pstride": 0}, INVALID), ({"q": ODD}, INVALID)])
+        ({"ppages": None}, INVALID), ({"rows": None}, INVALID), ({"pstride": 0}, INVALID),
+        ({"pstride": 1 << 27}, UNSUPPORTED), ({"q": ODD}, INVALID)])
 
 
 def test_window_prefill_refuses(native):

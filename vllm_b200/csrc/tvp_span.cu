@@ -20,6 +20,8 @@ int resolve_span_ctas(int num_ctas, int* out) {
   return tvp_device_sm_count(out);
 }
 
+constexpr int kMaxStride = INT_MAX / kPage;  // token positions are 32-bit
+
 bool span_heads_supported(int kv_heads) {
   return kv_heads == 1 || kv_heads == 2 || kv_heads == 4 || kv_heads == kMaxKvHeads;
 }
@@ -105,6 +107,7 @@ int tvp_paged_window_decode_attention(const tvp_bf16* q, const tvp_bf16* k_pool,
                              TVP_MODE_FAST, num_ctas);
   if (rc != TVP_OK) return rc;
   if (window < 1 || sinks < 0) return TVP_ERR_INVALID_ARGUMENT;
+  if (table_stride > kMaxStride) return TVP_ERR_UNSUPPORTED;
   int ctas = 0;
   if ((rc = resolve_span_ctas(num_ctas, &ctas)) != TVP_OK) return rc;
   const SpanWorkspace w = span_workspace(batch, 0, kv_heads, ctas);
@@ -135,6 +138,7 @@ int tvp_paged_shared_prefix_decode_attention(
   if (groups < 0 || groups > 65535 || prefix_stride < 0 || !aligned(q, 16) ||
       (groups > 0 && (!d_prefix_tables || !d_prefix_pages || !d_group_rows || prefix_stride < 1)))
     return TVP_ERR_INVALID_ARGUMENT;
+  if (table_stride > kMaxStride || prefix_stride > kMaxStride) return TVP_ERR_UNSUPPORTED;
   int ctas = 0;
   if ((rc = resolve_span_ctas(num_ctas, &ctas)) != TVP_OK) return rc;
   const SpanWorkspace w = span_workspace(batch, groups, kv_heads, ctas);
@@ -172,6 +176,7 @@ int tvp_paged_window_prefill_attention(const tvp_bf16* q, const tvp_bf16* k_pool
       num_seqs <= 0 || num_seqs > 65535 || max_q_len < 0 || window < 1 || sinks < 0 ||
       !std::isfinite(scale))
     return TVP_ERR_INVALID_ARGUMENT;
+  if (table_stride > kMaxStride) return TVP_ERR_UNSUPPORTED;
   if (max_q_len > 65535 * 32) return TVP_ERR_UNSUPPORTED;  // one grid row per 32-token tile
   if (!span_heads_supported(kv_heads) || q_heads != kv_heads * kGroup) return TVP_ERR_UNSUPPORTED;
   if ((long long)num_layers * num_pages * kPage > 0x7fffffffLL) return TVP_ERR_UNSUPPORTED;
