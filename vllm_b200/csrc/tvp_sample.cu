@@ -25,12 +25,14 @@
 // the 128 at the point.  For a small top-k the histogram is one of the largest
 // logits of every 32, which costs no pass over the row.
 //
-// What bounds it, at rows of 128256 logits: one row 8.5 us without filters, 11
-// with top-k 50, 27 with top-p 0.9 (launch, cluster barriers of about 1 us each,
-// and passes of one row over 8 SMs); 256 rows without filters 67 us (131 MB: 2.0
-// TB/s; the weights' FP64 arithmetic takes 50 of them), with top-k 50 47 us (2.8
-// TB/s, two passes of which one is from L2), with top-p 0.9 202 us (a weight
-// into a shared-memory histogram, two 32-bit atomics, for each logit with one).
+// What bounds it, at rows of 128256 logits: one row 8.1 us without filters, 10
+// with top-k 50, 24 with top-p 0.9 (launch, a chain of cluster barriers of about
+// 0.5 us and reads of other CTAs' shared memory, and passes of one row over 8
+// SMs); 256 rows without filters 68 us (131 MB: 1.9 TB/s; the weights' FP64
+// arithmetic takes 50 of them), with top-k 50 45 us (2.9 TB/s: the first pass
+// streams at the HBM rate, the chain behind it is the same as for one row), with
+// top-p 0.9 199 us (a weight into a shared-memory histogram, two 32-bit atomics,
+// for each logit with one).
 #include <cfloat>
 #include <climits>
 
@@ -96,7 +98,7 @@ struct alignas(16) Shared {
   double pow[256];
   Cut cut;
   Border border;
-  int fill;
+  int fill, hits;
   int part;  // where the draw's point lies, and the sum before
   u64 run;
 };
@@ -119,7 +121,7 @@ struct Powers {
 __device__ const Powers g_powers = Powers();
 
 constexpr size_t kScratchBytes = kBuckets * 8 + 5120;  // histogram, then the lists
-static_assert(kScratchBytes >= 3 * kList * 8, "the lists fit the histogram's place");
+static_assert(kScratchBytes >= 3 * kList * 8 + kList * 4, "the lists fit the histogram's place");
 static_assert(kScratchBytes >= (TVP_SAMPLE_MAX_VOCAB / 128 + 3) * 8, "and so do the sums");
 
 __host__ __device__ constexpr int batches_of(int logits) {
@@ -386,17 +388,28 @@ struct Sampler {
   __device__ u64* weights() const { return reinterpret_cast<u64*>(scratch) + 2 * kList; }
   __device__ int gather(int b0, int b1, int most) {
     u64* mine = reinterpret_cast<u64*>(scratch);
-    // A logit of bucket b1 lies above this (the distance is rounded, by 2^-23 of it
-    // at most, and so are the product and the quotient).
+    // A logit of bucket b1 lies above `floor`, one of b0 below `ceiling` (the distance
+    // is rounded, by 2^-23 of it at most, and so are the product and the quotient).
     const float reach =
         b1 < kBuckets - 1 && scale > 0.f ? (float)(b1 + 1) / scale * 1.000001f : INFINITY;
     const float floor = fmaxf(least, top - reach);
-    if (tid == 0) s.fill = 0;
+    const float ceiling = b0 > 0 ? top - (float)b0 / scale * 0.999999f : INFINITY;
+    int* hits = reinterpret_cast<int*>(weights() + kList);  // batches with a logit to list
+    if (tid == 0) s.fill = s.hits = 0;
     __syncthreads();
     if (b0 == 0) {  // at least one logit for each batch whose largest lies there
       int n = 0;
-      for (int it = 0; it < n_batches(); ++it) n += bucket(maxima[it * kThreads + tid]) <= b1 &&
-                                                    maxima[it * kThreads + tid] > least;
+      for (int it = 0; it < n_batches(); ++it) {
+        const float m = maxima[it * kThreads + tid];
+        const bool hit = bucket(m) <= b1 && m >= least;
+        n += hit && m > least;
+        const uint32_t all = __ballot_sync(0xffffffffu, hit);
+        if (all == 0) continue;
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&s.hits, __popc(all));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1u));
+        if (hit && at < kList) hits[at] = it * kThreads + tid;
+      }
       n = __reduce_add_sync(0xffffffffu, n);
       if (lane == 0 && n > 0) atomicAdd(&s.fill, n);
       __syncthreads();
@@ -406,18 +419,36 @@ struct Sampler {
       __syncthreads();
     }
     auto put = [&](float v, int i) {
-      if (!kept(v, begin + i) || bucket(v) < b0 || bucket(v) > b1) return;
+      if (v < floor || v > ceiling || !kept(v, begin + i) || bucket(v) < b0 || bucket(v) > b1) return;
       // past `most` the count no longer matters
       if (*const_cast<volatile int*>(&s.fill) > most) return;
       const int to = atomicAdd(&s.fill, 1);
       if (to < most) mine[to] = ((u64)order_of(v) << 32) | (uint32_t)~(begin + i);
     };
-    if (*const_cast<volatile int*>(&s.fill) <= most) each_four(floor, [&](const float4& v, int i) {
+    auto put4 = [&](const float4& v, int i) {
       put(v.x, i);
       put(v.y, i + 1);
       put(v.z, i + 2);
       put(v.w, i + 3);
-    });
+    };
+    if (*const_cast<volatile int*>(&s.fill) <= most) {
+      if (b0 == 0 && s.hits <= kList) {
+        // A few batches: a lane per quad, all of them at once.  (A warp that went
+        // over its own batches waited for L2 once per half batch: of 256 rows of
+        // top-k 50 each took 24 us, 17 this way.)
+        static_assert(kQuads == 8, "a lane per quad");
+        const float4* x4 = reinterpret_cast<const float4*>(x + head);
+        for (int j = tid / kQuads; j < s.hits; j += kThreads / kQuads) {
+          const int it = hits[j] / kThreads, owner = hits[j] % kThreads;
+          const int q = (it * kQuads + tid % kQuads) * kThreads + owner;
+          if (q < n_quads()) put4(x4[q], head + 4 * q);
+        }
+        const int i = single();
+        if (i >= 0) put(x[i], i);
+      } else {
+        each_four(floor, put4);
+      }
+    }
     __syncthreads();
     int* fills = s.fills[turn ^= 1];
     share(fills, s.fill);
@@ -613,6 +644,41 @@ struct Sampler {
   }
 };
 
+// The row that the turn-th cluster takes, where not all rows run at once: of
+// every kThreads rows first those that a histogram of weights goes over, then
+// those of a large top-k.  Such a row takes up to 78 us of its two CTAs, the others
+// 25; in the rows' own order the last of them to start ended 256 mixed rows at
+// 115 us.
+__device__ int in_turn(int turn, int rows, int vocab, const float* temperature,
+                       const int32_t* top_k, const float* top_p) {
+  __shared__ int counts[kWarps];  // rows of the first kind, and of the second << 16
+  __shared__ int found;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int base = turn / kThreads * kThreads, row = base + threadIdx.x;
+  const bool real = row < rows;
+  const float T = real && temperature ? __ldg(temperature + row) : 1.f;
+  const float P = real && top_p ? __ldg(top_p + row) : 1.f;
+  const int k = real && top_k ? __ldg(top_k + row) : 0;
+  const bool all = k <= 0 || k >= vocab;
+  const bool weighed = real && T > 0.f && all && P < 1.f;
+  const bool counted = real && T > 0.f && !all && k > kFew;
+  const uint32_t b0 = __ballot_sync(0xffffffffu, weighed), b1 = __ballot_sync(0xffffffffu, counted);
+  if (lane == 0) counts[warp] = __popc(b0) | __popc(b1) << 16;
+  __syncthreads();
+  const int upto = warp_scan(lane < kWarps ? counts[lane] : 0, lane);
+  const int total = __shfl_sync(0xffffffffu, upto, 31);
+  const int lower = warp > 0 ? __shfl_sync(0xffffffffu, upto, warp - 1) : 0;
+  const uint32_t mask = (1u << lane) - 1u;
+  const int before0 = (lower & 0xffff) + __popc(b0 & mask), before1 = (lower >> 16) + __popc(b1 & mask);
+  const int all0 = total & 0xffff, all1 = total >> 16;
+  const int place = weighed   ? before0
+                    : counted ? all0 + before1
+                              : all0 + all1 + (int)threadIdx.x - before0 - before1;
+  if (place == turn - base) found = row;
+  __syncthreads();
+  return found;
+}
+
 template <int CL, bool RES>
 __global__ void __launch_bounds__(kThreads, 2)
     sample_kernel(const float* __restrict__ logits, int vocab, int slice, long long row_stride,
@@ -621,8 +687,10 @@ __global__ void __launch_bounds__(kThreads, 2)
                   const float* __restrict__ min_p, int32_t* __restrict__ tokens) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Shared<CL> s;
-  const int rank = (int)cg::this_cluster().block_rank(), row = blockIdx.x / CL;
+  const int rank = (int)cg::this_cluster().block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = RES ? blockIdx.x / CL
+                      : in_turn(blockIdx.x / CL, gridDim.x / CL, vocab, temperature, top_k, top_p);
   const int begin = min(rank * slice, vocab), len = min(slice, vocab - begin);
   const float* src = logits + (size_t)row * row_stride + begin;
   // Logits before the first 16-byte boundary.
