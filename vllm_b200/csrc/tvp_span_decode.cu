@@ -395,13 +395,13 @@ __global__ void __launch_bounds__(Shape<KVH, SHARED>::kThreads, Shape<KVH, SHARE
 // from L2, a few microseconds for any batch.  (Folded by the decode kernel's
 // warps as they finished a row, the prefix pieces cost 2 to 3 us per row there,
 // with the pipeline standing.)
-constexpr int kMergeWarps = 8;
+constexpr int kMergeWarps = 4;  // of a block; 8: 256 rows 79.0 us instead of 78.0
 
 template <int KVH>
 __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const SpanParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool in_order = groups_in_order(p);
-  const int s = blockIdx.x * (kMergeWarps / KVH) + warp / KVH, h = warp % KVH;
+  const int at = blockIdx.x * kMergeWarps + warp, s = at / KVH, h = at % KVH;
   if (!in_order || s >= p.batch) return;
   // What the call's inputs say, before the launches before this one are done.
   const RowSpan span = decode_span<true>(p, s, false);
@@ -410,15 +410,15 @@ __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const Sp
   asm volatile("griddepcontrol.wait;" ::: "memory");
   Fold f;
   // The prefix's pieces, then the row's own; both counts in one round trip.
-  const int2 at = g >= 0 ? __ldcg(p.group_pieces + g) : make_int2(0, 0);
+  const int2 in = g >= 0 ? __ldcg(p.group_pieces + g) : make_int2(0, 0);
   const int2 r = span.pages > 0 ? __ldcg(p.row_ranges + s) : make_int2(0, -1);
-  const float* shared = p.pieces + ((size_t)(at.x + ((t / kTileRows) * KVH + h) * at.y) * kTileRows +
+  const float* shared = p.pieces + ((size_t)(in.x + ((t / kTileRows) * KVH + h) * in.y) * kTileRows +
                                     t % kTileRows) * kPartialFloats;
   const float* own = p.partials + ((size_t)(s + r.x) * KVH + h) * kPartialFloats;
-  f.add_all(at.y + r.y - r.x + 1,
+  f.add_all(in.y + r.y - r.x + 1,
             [&](int i) {
-              return i < at.y ? shared + (size_t)i * kPieceFloats
-                              : own + (size_t)(i - at.y) * KVH * kPartialFloats;
+              return i < in.y ? shared + (size_t)i * kPieceFloats
+                              : own + (size_t)(i - in.y) * KVH * kPartialFloats;
             },
             lane);
   f.write(p.out + ((size_t)s * KVH + h) * kGroup * kHeadDim, lane);
@@ -478,7 +478,7 @@ cudaError_t launch_heads(const SpanParams& p, const CUtensorMap& k_map, const CU
 template <int KVH>
 cudaError_t launch_merge(const SpanParams& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.batch + kMergeWarps / KVH - 1) / (kMergeWarps / KVH)));
+  cfg.gridDim = dim3((unsigned)(((long long)p.batch * KVH + kMergeWarps - 1) / kMergeWarps));
   cfg.blockDim = dim3(kMergeWarps * 32);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
