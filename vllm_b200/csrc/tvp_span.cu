@@ -32,8 +32,8 @@ struct SpanWorkspace {
 };
 
 // counters[1024][8] | row_ranges[batch] | group_pieces[groups] | partials | pieces.
-// The counters' place and size are the same for every call.  Pieces: two CTAs
-// per SM, or one per tile of 32 rows and KV head where those are more.
+// The counters' place and size are the same for every call.  Pieces: one
+// per CTA, or per tile of 32 rows and KV head where those are more.
 SpanWorkspace span_workspace(int batch, int groups, int kv_heads, int num_ctas) {
   auto align = [](size_t x) { return (x + 255) / 256 * 256; };
   SpanWorkspace w = {};
@@ -44,7 +44,7 @@ SpanWorkspace span_workspace(int batch, int groups, int kv_heads, int num_ctas) 
   w.pieces = align(w.partials + slots * kv_heads * kPartialFloats * 4);
   if (groups > 0) {
     const int streams = kv_heads * (batch / kTileRows + groups);
-    w.max_pieces = streams > 2 * num_ctas ? streams : 2 * num_ctas;
+    w.max_pieces = streams > num_ctas ? streams : num_ctas;
   }
   w.total = align(w.pieces + (size_t)w.max_pieces * kPieceFloats * 4);
   return w;
@@ -75,7 +75,7 @@ void fill_workspace(void* d_workspace, const SpanWorkspace& w, int num_ctas, Spa
   p->group_pieces = reinterpret_cast<int2*>(base + w.group_pieces);
   p->partials = reinterpret_cast<float*>(base + w.partials);
   p->pieces = reinterpret_cast<float*>(base + w.pieces);
-  p->piece_target = 2 * num_ctas;
+  p->piece_target = num_ctas;
 }
 
 int map_cuda(cudaError_t e) { return e == cudaSuccess ? TVP_OK : TVP_ERR_RUNTIME; }

@@ -58,7 +58,7 @@ struct Fold {
     o[6] = o[6] * wa + b.z * wb; o[7] = o[7] * wa + b.w * wb;
   }
   // n partials, the i-th at at(i), kFlight in flight at once, folded in order.
-  static constexpr int kFlight = 6;
+  static constexpr int kFlight = 8;
   template <typename At>
   __device__ __forceinline__ void add_all(int n, At at, int lane) {
     const int h = lane >> 3, d = 2 * kGroup + h * kHeadDim + (lane & 7) * 8;

@@ -5,7 +5,9 @@
 //   * PREFIX: the 32 tokens are 32 rows of a group, the pages a part of its
 //     prefix ("piece"); the CTA leaves (m, l, O) per (row, head) for the merge
 //     kernel to fold in.  The pieces' length is the shortest that keeps their
-//     number within piece_target (two CTAs per SM), so a few long prefixes and
+//     number within piece_target (one CTA per SM, next to the decode kernel's: two
+//     pieces per SM, one after the other, took 26.7 us instead of 18.2 for 8 rows
+//     behind 8192 tokens, 78 instead of 75 for 256), so a few long prefixes and
 //     many short ones both fill the GPU once; every CTA works this out from the
 //     group sizes, a search of some ten steps by one warp.
 //   * window: the tokens are a tile of a sequence's queries, the pages the ones
@@ -166,11 +168,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int32_t* table;
   if (PREFIX) {
     // Launched beside the decode kernel (a programmatic dependent launch that
-    // needs nothing of it).  The merge kernel waits for this grid alone, so one
-    // block of it, which has a piece only when there are as many as fit, waits
-    // for the decode kernel.
+    // needs nothing of it).  The merge kernel waits for this grid alone, so its
+    // last block, behind the ones that may have a piece, waits for the decode
+    // kernel.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (blockIdx.x == gridDim.x - 1) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      return;
+    }
     if (!groups_in_order(p)) return;  // the decode kernel reports it
     Piece* shared_piece = reinterpret_cast<Piece*>(smem + kOffPlan);
     if (warp == 0) {
@@ -638,7 +643,7 @@ cudaError_t launch_tiles(const SpanParams& p, long long pool_rows, dim3 grid, cu
 
 cudaError_t launch_prefix_tiles(const SpanParams& p, long long pool_rows, int max_pieces,
                                 cudaStream_t stream) {
-  return launch_tiles<true>(p, pool_rows, dim3((unsigned)max_pieces), stream);
+  return launch_tiles<true>(p, pool_rows, dim3((unsigned)max_pieces + 1), stream);
 }
 
 cudaError_t launch_window_tiles(const SpanParams& p, long long pool_rows, int max_q_len,
