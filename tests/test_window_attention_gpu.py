@@ -100,6 +100,20 @@ def test_whole_window_equals_plain_decode_attention():
     S.check(got, case)
 
 
+def test_windows_and_sinks_past_32_bits_see_everything():
+    case = S.SpanCase(51, [300, 17], window=1 << 30, sinks=0)
+    for window, sinks in ((1 << 33, 0), (1, (1 << 32) + 1)):
+        case.window, case.sinks = window, sinks
+        got, err = run_decode(case)
+        assert err == 0
+        S.check(got, case)
+    prompt = S.SpanCase(52, [70], window=1 << 30, sinks=0, q_counts=[70])
+    prompt.window = (1 << 32) + 2
+    got, err = run_prefill(prompt)
+    assert err == 0
+    S.check(got, prompt)
+
+
 def test_decode_bad_pages_and_lengths_are_reported():
     case = S.SpanCase(60, [300, 60, 45], window=100, sinks=4)
     ok, _ = run_decode(case)

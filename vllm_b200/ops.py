@@ -279,34 +279,32 @@ class _Call:
     __slots__ = ("dev", "stream", "given", "before")
 
     def __init__(self, dev, stream):
-        if stream is not None and stream.device != dev:
-            raise ValueError(f"stream is of {stream.device}, the tensors are on {dev}")
         self.dev, self.given = dev, stream
+        if stream is not None:
+            if stream.device != dev:
+                raise ValueError(f"stream is of {stream.device}, the tensors are on {dev}")
+            self.stream = stream.cuda_stream
+        else:
+            # the raw handle: making a Stream object of it takes 4 us
+            self.stream = torch._C._cuda_getCurrentRawStream(dev.index)
 
     def __enter__(self):
-        self.before = torch.cuda.current_device()
+        self.before = torch._C._cuda_getDevice()
         if self.before != self.dev.index:
             torch.cuda.set_device(self.dev)
-        # the raw handle: making a Stream object of it takes 4 us
-        self.stream = (torch._C._cuda_getCurrentRawStream(self.dev.index) if self.given is None
-                       else self.given.cuda_stream)
         return self
 
     def __exit__(self, *exc):
         if self.before != self.dev.index:
             torch.cuda.set_device(self.before)
 
-    def empty_like(self, like, dtype):
-        """A tensor that belongs to the call's stream."""
-        if self.given is None:
-            return torch.empty_like(like, dtype=dtype)
-        with torch.cuda.stream(self.given):
-            return torch.empty_like(like, dtype=dtype)
-
     def output(self, out, like, dtype):
-        """``out``, or a tensor shaped like ``like``."""
+        """``out``, or a tensor shaped like ``like`` that belongs to the call's stream."""
         if out is None:
-            return self.empty_like(like, dtype)
+            if self.given is None:
+                return torch.empty_like(like, dtype=dtype)
+            with torch.cuda.stream(self.given):
+                return torch.empty_like(like, dtype=dtype)
         _take(out, "out", dtype, self.dev)
         if out.shape != like.shape:
             raise ValueError(f"out must be {list(like.shape)}")
@@ -314,17 +312,22 @@ class _Call:
 
 
 def _span_geometry(k_pool, v_pool, q, block_tables, error):
-    """Argument checks that the span calls share; the pools' geometry."""
-    dev = k_pool.device
-    if k_pool.get_device() < 0:
-        _need(k_pool, "k_pool", torch.bfloat16)
-    _take(k_pool, "k_pool", torch.bfloat16, dev)
-    _take(v_pool, "v_pool", torch.bfloat16, dev)
-    shape = k_pool.shape
+    """Argument checks that the span calls share; the device and the pools' geometry."""
+    bf16, at = torch.bfloat16, k_pool.get_device()
+    # one test where all is well (the calls' host time is what a small batch takes)
+    if q is None or v_pool is None or block_tables is None or at < 0 or \
+            not (k_pool.dtype is bf16 and v_pool.dtype is bf16 and q.dtype is bf16
+                 and block_tables.dtype is torch.int32
+                 and at == v_pool.get_device() == q.get_device() == block_tables.get_device()
+                 and k_pool.is_contiguous() and v_pool.is_contiguous() and q.is_contiguous()
+                 and block_tables.is_contiguous()):
+        _need(k_pool, "k_pool", bf16)
+        for t, name in ((v_pool, "v_pool"), (q, "q")):
+            _need(t, name, bf16, k_pool.device)
+        _need(block_tables, "block_tables", torch.int32, k_pool.device)
+    dev, shape = k_pool.device, k_pool.shape
     if len(shape) != 4 or shape != v_pool.shape or shape[2] != N.PAGE_TOKENS or shape[3] % N.HEAD_DIM:
         raise ValueError("pools must be [num_layers, num_pages, 16, kv_heads*64] and equal")
-    _take(q, "q", torch.bfloat16, dev)
-    _take(block_tables, "block_tables", torch.int32, dev)
     if error is not None:
         _take(error, "error", torch.int32, dev)
     if q.dim() != 2 or q.shape[1] != shape[3] * N.GQA_GROUP:
@@ -332,6 +335,14 @@ def _span_geometry(k_pool, v_pool, q, block_tables, error):
     if block_tables.dim() != 2:
         raise ValueError("block_tables must be [rows, table_stride]")
     return dev, shape[0], shape[1], shape[3] // N.HEAD_DIM
+
+
+def _window(window, sinks):
+    """Window and sinks as the 32-bit counts of a call; no length passes 32 bits."""
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError("window must be at least 1, sinks at least 0")
+    return min(window, 0x7fffffff), min(sinks, 0x7fffffff)
 
 
 def _decode_rows(kv_heads, dev, q, block_tables, seq_lens, workspace):
@@ -361,13 +372,14 @@ def paged_window_decode_attention(q, k_pool, v_pool, layer, block_tables, seq_le
     lib = N.load()
     dev, num_layers, num_pages, kv_heads = _span_geometry(k_pool, v_pool, q, block_tables, error)
     batch = _decode_rows(kv_heads, dev, q, block_tables, seq_lens, workspace)
+    window, sinks = _window(window, sinks)
     with _Call(dev, stream) as call:
         out = call.output(out, q, torch.bfloat16)
         rc = lib.tvp_paged_window_decode_attention(
-            _addr(q), _addr(k_pool), _addr(v_pool), num_pages, num_layers, layer, kv_heads,
-            kv_heads * N.GQA_GROUP, _addr(block_tables), block_tables.shape[1], _addr(seq_lens),
-            batch, int(window), int(sinks), float(scale), workspace.num_ctas,
-            _addr(workspace.buffer), workspace.nbytes, _addr(out), _addr(error), call.stream)
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), num_pages, num_layers, layer, kv_heads,
+            kv_heads * N.GQA_GROUP, block_tables.data_ptr(), block_tables.shape[1], seq_lens.data_ptr(),
+            batch, window, sinks, float(scale), workspace.num_ctas,
+            workspace.buffer.data_ptr(), workspace.nbytes, out.data_ptr(), _addr(error), call.stream)
     N.check(rc, "tvp_paged_window_decode_attention")
     return out
 
@@ -397,11 +409,11 @@ def paged_shared_prefix_decode_attention(q, k_pool, v_pool, layer, block_tables,
     with _Call(dev, stream) as call:
         out = call.output(out, q, torch.bfloat16)
         rc = lib.tvp_paged_shared_prefix_decode_attention(
-            _addr(q), _addr(k_pool), _addr(v_pool), num_pages, num_layers, layer, kv_heads,
-            kv_heads * N.GQA_GROUP, _addr(block_tables), block_tables.shape[1], _addr(seq_lens),
-            batch, _addr(prefix_tables), prefix_tables.shape[1], _addr(prefix_pages),
-            _addr(group_rows), groups, float(scale), workspace.num_ctas, _addr(workspace.buffer),
-            workspace.nbytes, _addr(out), _addr(error), call.stream)
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), num_pages, num_layers, layer, kv_heads,
+            kv_heads * N.GQA_GROUP, block_tables.data_ptr(), block_tables.shape[1], seq_lens.data_ptr(),
+            batch, prefix_tables.data_ptr(), prefix_tables.shape[1], prefix_pages.data_ptr(),
+            group_rows.data_ptr(), groups, float(scale), workspace.num_ctas, workspace.buffer.data_ptr(),
+            workspace.nbytes, out.data_ptr(), _addr(error), call.stream)
     N.check(rc, "tvp_paged_shared_prefix_decode_attention")
     return out
 
@@ -420,15 +432,16 @@ def paged_window_prefill_attention(q, k_pool, v_pool, layer, block_tables, cu_q,
         raise ValueError("cu_q must have num_seqs + 1 entries")
     if block_tables.shape[0] < num_seqs:
         raise ValueError("block_tables must be [>=num_seqs, table_stride]")
+    window, sinks = _window(window, sinks)
     with _Call(dev, stream) as call:
         out = call.output(out, q, torch.bfloat16)
         if q.shape[0] == 0:
             return out
         rc = lib.tvp_paged_window_prefill_attention(
-            _addr(q), _addr(k_pool), _addr(v_pool), num_pages, num_layers, layer, kv_heads,
-            kv_heads * N.GQA_GROUP, _addr(block_tables), block_tables.shape[1], _addr(cu_q),
-            _addr(q_pos0), num_seqs, int(max_q_len), int(window), int(sinks), float(scale),
-            _addr(out), _addr(error), call.stream)
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), num_pages, num_layers, layer, kv_heads,
+            kv_heads * N.GQA_GROUP, block_tables.data_ptr(), block_tables.shape[1], cu_q.data_ptr(),
+            q_pos0.data_ptr(), num_seqs, int(max_q_len), window, sinks, float(scale),
+            out.data_ptr(), _addr(error), call.stream)
     N.check(rc, "tvp_paged_window_prefill_attention")
     return out
 
@@ -461,9 +474,9 @@ def sample_tokens(logits, uniforms, temperature=None, top_k=None, top_p=None, mi
             raise ValueError(f"{name} must have one entry per row")
     with _Call(dev, stream) as call:
         out = call.output(out, uniforms, torch.int32)
-        rc = lib.tvp_sample_tokens(_addr(logits), rows, vocab, max(logits.stride(0), vocab),
-                                   _addr(uniforms), _addr(temperature), _addr(top_k), _addr(top_p),
-                                   _addr(min_p), _addr(out), call.stream)
+        rc = lib.tvp_sample_tokens(logits.data_ptr(), rows, vocab, max(logits.stride(0), vocab),
+                                   uniforms.data_ptr(), _addr(temperature), _addr(top_k), _addr(top_p),
+                                   _addr(min_p), out.data_ptr(), call.stream)
     N.check(rc, "tvp_sample_tokens")
     return out
 
