@@ -62,9 +62,14 @@ static_assert(kBlocks == 64 && kBuckets / kCluster % 32 == 0, "border() deals th
 constexpr int kStreamRows = 64;
 constexpr int kStreamMany = 192;
 constexpr int kList = 512;  // logits of a bucket that CTA 0 takes in
-// Logits at or above the cut that CTA 0 finishes by itself.  Each-with-each takes
-// 2 x 0.7 us for 128 and 2 x 11 us for 512; the sums take some 3 us of passes.
-constexpr int kFew = 160;
+// Logits at or above the cut that CTA 0 finishes by itself, each compared with
+// each by two threads or more per logit.  Top-k 200 that way: one row 14.4 us, 256
+// rows 63; by the cut and sums 17.5 and 105.  Above 256 a logit has one thread, and
+// 512 took 22 us.
+constexpr int kFew = 256;
+// The largest top-k that starts on this way: the list holds some more than k
+// logits, and one that overflows costs 6 to 9 us.
+constexpr int kFewK = 224;
 constexpr int kFixedBits = 44;
 // A distance (in units of T) where a weight rounds to 0: 45 ln 2 is 31.2, and
 // the subtraction's rounding takes half a last place of the top.
@@ -616,7 +621,7 @@ struct Sampler {
     auto any = [](float) { return true; };
     auto bin = [&](float v) { return bucket(v); };
     auto want = [&](u64 total) { return MASS ? want_of(P, total) : (u64)k; };
-    if (!MASS && k <= kFew) {
+    if (!MASS && k <= kFewK) {
       // The k-th largest of the batches' maxima is no larger than the k-th
       // largest logit: what lies above it holds the k, and little more.
       const Border edge = border<false, true>(any, bin, want);
@@ -630,7 +635,7 @@ struct Sampler {
     }
     const Border edge = border<MASS, false>(any, bin, want);
     if (edge.bin == kBuckets) return false;  // fewer logits with a weight than k
-    if (MASS || k <= kFew) {
+    if (MASS || k <= kFewK) {
       // After a histogram of weights the amount wanted is known, of the whole;
       // after one of counts, top-p is of the k that are left.
       const int n = gather(0, edge.bin, kFew);
@@ -661,7 +666,7 @@ __device__ int in_turn(int turn, int rows, int vocab, const float* temperature,
   const int k = real && top_k ? __ldg(top_k + row) : 0;
   const bool all = k <= 0 || k >= vocab;
   const bool weighed = real && T > 0.f && all && P < 1.f;
-  const bool counted = real && T > 0.f && !all && k > kFew;
+  const bool counted = real && T > 0.f && !all && k > kFewK;
   const uint32_t b0 = __ballot_sync(0xffffffffu, weighed), b1 = __ballot_sync(0xffffffffu, counted);
   if (lane == 0) counts[warp] = __popc(b0) | __popc(b1) << 16;
   __syncthreads();
