@@ -43,6 +43,29 @@ def test_random_rows(vocab, rows):
         check(x, rng.random(rows), **settings_of(rng, rows, min(vocab, 500)))
 
 
+@pytest.mark.parametrize("vocab", [65535, 65536, 65539, 327680])
+@pytest.mark.parametrize("rows", [1, 4])
+def test_few_rows_of_large_vocabularies(vocab, rows):
+    """Both sides of the sizes where a row gets the larger cluster."""
+    rng = np.random.default_rng(vocab + rows)
+    x = (rng.standard_normal((rows, vocab)) * 2.5).astype(np.float32)
+    x[:, rng.integers(0, vocab, 20)] += 8
+    x[0, 1::2] = np.round(x[0, 1::2])  # ties at every cut
+    for k_hi in (200, 5000):
+        check(x, rng.random(rows), **settings_of(rng, rows, k_hi))
+    check(x, rng.random(rows), top_p=np.full(rows, 0.9))
+    check(x, rng.random(rows), top_k=np.full(rows, 3000), min_p=np.full(rows, 0.01))
+
+
+@pytest.mark.parametrize("k", [160, 161, 223, 224, 225, 256, 257])
+def test_top_k_around_the_lists_sizes(k):
+    rng = np.random.default_rng(k)
+    for rows in (2, 80, 200):
+        x = (rng.standard_normal((rows, 30000)) * 2).astype(np.float32)
+        x[::2] = np.round(x[::2] * 8) / 8  # ties
+        check(x, rng.random(rows), top_k=np.full(rows, k), top_p=rng.choice([1.0, 0.8], rows))
+
+
 def test_many_rows():
     rng = np.random.default_rng(3)
     x = (rng.standard_normal((300, 2000)) * 2).astype(np.float32)

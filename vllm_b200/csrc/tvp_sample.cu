@@ -1,7 +1,7 @@
 // K9 — one token per row of logits from given random numbers.
 //
-// A cluster of CTAs takes a row: 8 that keep the logits in shared memory while
-// there are few rows, so that a row is read once from HBM however many passes
+// A cluster of CTAs takes a row: 8 or 16 that keep the logits in shared memory
+// while there are few rows, so that a row is read once from HBM however many passes
 // the filters take, and 4 or 2 that read them again from L2 when there are many
 // (kStreamRows).
 //
@@ -26,8 +26,8 @@
 // logits of every 32, which costs no pass over the row.
 //
 // What bounds it, at rows of 128256 logits: one row 8.1 us without filters, 10
-// with top-k 50, 24 with top-p 0.9 (launch, a chain of cluster barriers of about
-// 0.5 us and reads of other CTAs' shared memory, and passes of one row over 8
+// with top-k 50, 22 with top-p 0.9 (launch, a chain of cluster barriers of about
+// 0.5 us and reads of other CTAs' shared memory, and passes of one row over 16
 // SMs); 256 rows without filters 68 us (131 MB: 1.9 TB/s; the weights' FP64
 // arithmetic takes 50 of them), with top-k 50 45 us (2.9 TB/s: the first pass
 // streams at the HBM rate, the chain behind it is the same as for one row), with
@@ -52,13 +52,20 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBuckets = 2048;
 constexpr int kQuads = 8;  // fours of logits per batch of a thread
 constexpr int kBlocks = kBuckets / 32;  // two per lane of a warp
-static_assert(kBlocks == 64 && kBuckets / kCluster % 32 == 0, "border() deals them out so");
 // Few rows: 8 CTAs keep a row in shared memory.  From kStreamRows on, 4 CTAs per
 // row read it again from L2 (kStreamMany: 2), which leaves room for more rows at
 // once.  Measured, us for rows of 128256 of mixed settings, 8 kept / 4 / 2
 // streaming: 32 rows 32 / 46 / 76, 64 rows 50 / 51 / 77, 96 rows 69 / 60 / 71,
 // 256 rows 157 / 115 / 117; of top-k 50: 32 rows 14 / 14 / 17, 64 rows
 // 27 / 16 / 17, 256 rows 105 / 65 / 47.
+// A few rows of a large vocabulary: 16 CTAs.  One row, top-p 0.9, 8 CTAs / 16: of
+// 300000 logits 51 / 37 us, of 128256 25 / 22, of 50257 20.5 / 20.2, of 1000
+// 9.7 / 10.3 (a larger cluster's barriers take longer); 8 rows of 128256 27.9 / 27.4
+// and without filters 8.7 / 12.0, as eight such clusters do not start at once.
+constexpr int kWide = 16;
+constexpr int kWideRows = 4;
+constexpr int kWideVocab = 65536;
+static_assert(kBlocks == 64 && kBuckets / kWide % 32 == 0, "border() deals them out so");
 constexpr int kStreamRows = 64;
 constexpr int kStreamMany = 192;
 constexpr int kList = 512;  // logits of a bucket that CTA 0 takes in
@@ -960,16 +967,6 @@ cudaError_t launch_sampler(int rows, int vocab, long long row_stride, const floa
   auto smem_of = [](int slice) {
     return kScratchBytes + (size_t)batches_of(slice) * kThreads * 4 + (RES ? (size_t)slice * 4 + 16 : 0);
   };
-  static bool configured[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(sample_kernel<CL, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)smem_of(slice_of(TVP_SAMPLE_MAX_VOCAB)));
-    if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) configured[dev] = true;
-  }
   const int slice = slice_of(vocab);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * CL);
@@ -982,6 +979,30 @@ cudaError_t launch_sampler(int rows, int vocab, long long row_stride, const floa
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  static bool configured[64] = {}, unfit[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    const size_t most = smem_of(slice_of(TVP_SAMPLE_MAX_VOCAB));
+    e = cudaFuncSetAttribute(sample_kernel<CL, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)most);
+    if (e != cudaSuccess) return e;
+    if (CL > kCluster) {  // more than every device takes: only where one has room
+      e = cudaFuncSetAttribute(sample_kernel<CL, RES>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return e;
+      cudaLaunchConfig_t largest = cfg;
+      largest.gridDim = dim3(CL);
+      largest.dynamicSmemBytes = most;
+      int clusters = 0;
+      e = cudaOccupancyMaxActiveClusters(&clusters, sample_kernel<CL, RES>, &largest);
+      if (e != cudaSuccess) return e;
+      if (clusters < 1 && (dev < 0 || dev >= 64)) return cudaErrorNotSupported;
+      if (clusters < 1) unfit[dev] = true;
+    }
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  if (dev >= 0 && dev < 64 && unfit[dev]) return cudaErrorNotSupported;
   return cudaLaunchKernelEx(&cfg, sample_kernel<CL, RES>, logits, vocab, slice, row_stride, uniforms,
                             temperature, top_k, top_p, min_p, tokens);
 }
@@ -997,10 +1018,15 @@ extern "C" int tvp_sample_tokens(const float* d_logits, int rows, int vocab, lon
     return TVP_ERR_INVALID_ARGUMENT;
   if (vocab > TVP_SAMPLE_MAX_VOCAB || rows > 65535) return TVP_ERR_UNSUPPORTED;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const auto launch = rows < kStreamRows   ? launch_sampler<kCluster, true>
-                      : rows < kStreamMany ? launch_sampler<4, false>
-                                           : launch_sampler<2, false>;
-  const cudaError_t e = launch(rows, vocab, row_stride, d_logits, d_uniforms, d_temperature,
-                               d_top_k, d_top_p, d_min_p, d_tokens, st);
+  auto run = [&](auto launch) {
+    return launch(rows, vocab, row_stride, d_logits, d_uniforms, d_temperature, d_top_k, d_top_p,
+                  d_min_p, d_tokens, st);
+  };
+  cudaError_t e = cudaErrorNotSupported;
+  if (rows <= kWideRows && vocab >= kWideVocab) e = run(launch_sampler<kWide, true>);
+  if (e == cudaErrorNotSupported)
+    e = run(rows < kStreamRows   ? launch_sampler<kCluster, true>
+            : rows < kStreamMany ? launch_sampler<4, false>
+                                 : launch_sampler<2, false>);
   return e == cudaSuccess ? TVP_OK : TVP_ERR_RUNTIME;
 }
