@@ -72,6 +72,20 @@ def test_many_rows():
     check(x, rng.random(300), **settings_of(rng, 300, 100))
 
 
+def test_more_rows_than_are_put_in_turn_at_once():
+    rng = np.random.default_rng(13)
+    x = (rng.standard_normal((1100, 900)) * 2).astype(np.float32)
+    check(x, rng.random(1100), **settings_of(rng, 1100, 400))
+
+
+@pytest.mark.parametrize("only", ["temperature", "top_k", "top_p", "min_p", None])
+def test_each_setting_alone_of_many_rows(only):
+    rng = np.random.default_rng(14)
+    x = (rng.standard_normal((200, 3000)) * 2).astype(np.float32)
+    s = settings_of(rng, 200, 400)
+    check(x, rng.random(200), **({only: s[only]} if only else {}))
+
+
 @pytest.mark.parametrize("only", ["temperature", "top_k", "top_p", "min_p", None])
 def test_each_setting_alone(only):
     rng = np.random.default_rng(4)
