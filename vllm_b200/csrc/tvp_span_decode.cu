@@ -59,7 +59,8 @@ struct Fold {
     o[4] = o[4] * wa + b.x * wb; o[5] = o[5] * wa + b.y * wb;
     o[6] = o[6] * wa + b.z * wb; o[7] = o[7] * wa + b.w * wb;
   }
-  // n partials, the i-th at at(i), kFlight in flight at once, folded in order.
+  // n partials, the i-th at at(i), kFlight in flight at once, folded in order (256
+  // rows behind 8192 tokens: 76.9 us with 8, 77.6 with 6, 80.4 with 4, 78.4 with 10).
   static constexpr int kFlight = 8;
   template <typename At>
   __device__ __forceinline__ void add_all(int n, At at, int lane) {

@@ -51,7 +51,9 @@ constexpr uint32_t kColP = 64, kColO = 128;
 constexpr int kLowRegs = 32;    // warps 0-3
 constexpr int kHighRegs = 104;  // the softmax warps
 constexpr unsigned kProducerNs = 200, kMmaNs = 40;  // sleeps of the waiting warps
-constexpr int kMinChunks = 2;   // a piece of a prefix is no shorter than this
+// A piece of a prefix is no shorter than this: 4 rows behind 512 tokens take 12.2 us
+// with 2 chunks, 12.8 with 4; one chunk each made 32 rows behind 1024 tokens 12% slower.
+constexpr int kMinChunks = 2;
 
 constexpr int kOffStages = kQBytes;
 constexpr int kOffBars = kOffStages + kStages * kChunkBytes;
