@@ -35,6 +35,7 @@
 // for each logit with one).
 #include <cfloat>
 #include <climits>
+#include <utility>
 
 #include <cooperative_groups.h>
 
@@ -699,6 +700,10 @@ __global__ void __launch_bounds__(kThreads, 2)
                   const float* __restrict__ min_p, int32_t* __restrict__ tokens) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Shared<CL> s;
+  // Another CTA's shared memory may be written once that CTA is known to run: every
+  // CTA says so here, and waits for the others before its first remote store, with
+  // the first pass over the row in between.
+  auto started = cg::this_cluster().barrier_arrive();
   const int rank = (int)cg::this_cluster().block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = RES ? blockIdx.x / CL
@@ -765,6 +770,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     top = fmaxf(top, s.warp_most[w]);
     lo = fminf(lo, s.warp_least[w]);
   }
+  cg::this_cluster().barrier_wait(std::move(started));
   if (tid < CL) {
     Sampler<CL, RES>::of_rank(s.most, tid)[rank] = top;
     Sampler<CL, RES>::of_rank(s.least, tid)[rank] = lo;
