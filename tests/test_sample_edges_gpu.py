@@ -37,3 +37,25 @@ def test_rows_shorter_than_their_cluster(rows, vocab):
         got = [ops.sample_tokens(xs, us, top_k=ks) for _ in range(20)]
         for g in got:
             assert g.tolist() == [w for w, _ in want]
+
+
+@pytest.mark.parametrize("rows", [1, 8, 70, 200])
+@pytest.mark.parametrize("top", [1e7, 20.0, -3.5])
+@pytest.mark.parametrize("step", [0.04, 0.045, 0.075, 0.2])
+def test_temperatures_below_the_tops_last_place(rows, top, step):
+    """Temperature `step` of the top's last place: every logit but the top is more than
+    20 of these steps lower and has no weight, whatever the subtraction that finds
+    the first such logit rounds to; so every uniform takes the top, first or last of its row."""
+    vocab = 70001
+    rng = np.random.default_rng(rows)
+    top = np.float32(top)
+    x = (top - np.float32(4) * np.spacing(np.abs(top)) * rng.integers(20, 1 << 18, (rows, vocab))).astype(np.float32)
+    x[:, 7::13] = -np.inf
+    x[:, 9::17] = np.nan
+    at = np.where(np.arange(rows) % 2 == 0, 0, vocab - 1)
+    x[np.arange(rows), at] = top
+    t = np.full(rows, step * np.spacing(np.abs(top)))
+    near = np.where(at == 0, np.float32(1 - 2.0 ** -24), np.float32(1e-6))
+    for settings in ({}, {"top_k": np.full(rows, 3)}, {"top_p": np.full(rows, 0.9)}, {"min_p": np.full(rows, 1e-6)}):
+        for u in (near, 1 - near, np.full(rows, 0.5)):
+            assert draw(x, u, temperature=t, **settings).tolist() == at.tolist(), settings

@@ -79,8 +79,7 @@ constexpr int kFew = 256;
 // logits, and one that overflows costs 6 to 9 us.
 constexpr int kFewK = 224;
 constexpr int kFixedBits = 44;
-// A distance (in units of T) where a weight rounds to 0: 45 ln 2 is 31.2, and
-// the subtraction's rounding takes half a last place of the top.
+// A distance (in units of T) where a weight rounds to 0: from 45 ln 2 = 31.2 on.
 constexpr float kFar = 33.f;
 constexpr double kTwo52 = 4503599627370496.0;
 
@@ -841,7 +840,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   // weight 0 as that 512th does, and keeps the distances' exponents in range.
   const float under = nextafterf(top, -INFINITY);
   T = fmaxf(T, (top - under) * (1.f / 512.f));
-  const float far = fmaxf(fminf(top - kFar * T, under), -FLT_MAX);
+  // Rounded away from the top: to the nearest, a T of 0.045 of the top's last place left
+  // `far` 22 T below it, where a weight is 3929 of 2^-44.
+  const float far = fmaxf(fminf(__fsub_rd(top, __fmul_ru(kFar, T)), under), -FLT_MAX);
   // Buckets over the distances that have weight, or over the row's own range
   // where that is narrower (and not a masked row's, whose least is -inf).
   const float range = fminf(kFar * T, top - lo);
