@@ -59,3 +59,27 @@ def test_temperatures_below_the_tops_last_place(rows, top, step):
     for settings in ({}, {"top_k": np.full(rows, 3)}, {"top_p": np.full(rows, 0.9)}, {"min_p": np.full(rows, 1e-6)}):
         for u in (near, 1 - near, np.full(rows, 0.5)):
             assert draw(x, u, temperature=t, **settings).tolist() == at.tolist(), settings
+
+
+@pytest.mark.parametrize("rows", [1, 8, 70, 200])
+@pytest.mark.parametrize("exponent", [-119, -125, -135, -142])
+def test_tiny_logits_and_temperatures(rows, exponent):
+    """Logits and temperature scaled by a power of two, down to subnormal ones, draw what the
+    unscaled ones do: only their quotient counts.  (Logits are multiples of 2^-6: exact.)"""
+    vocab = 70001
+    rng = np.random.default_rng(rows - exponent)
+    x = np.round(rng.standard_normal((rows, vocab)) * 200).astype(np.float32) / 64
+    scaled = np.ldexp(x, exponent)
+    assert np.array_equal(np.ldexp(scaled.astype(np.float64), -exponent), x)
+    temperature = rng.choice([0.25, 0.5, 1.0, 2.0], rows).astype(np.float32)
+    for s in ({}, {"top_k": rng.integers(1, 3000, rows)}, {"top_p": rng.choice([0.3, 0.9], rows)},
+              {"min_p": rng.choice([0.05, 0.3, 0.999], rows)}):
+        u, want = rng.random(rows).astype(np.float32), np.zeros(rows, int)
+        for r in range(rows):
+            one = {k: (int if k == "top_k" else np.float32)(v[r]) for k, v in s.items()}
+            want[r], near = sample_row(x[r], u[r], temperature[r], **one)
+            while near <= vocab * 2.0 ** -43:  # the weights' rounding decides: another draw
+                u[r] = rng.random()
+                want[r], near = sample_row(x[r], u[r], temperature[r], **one)
+        got = draw(scaled, u, temperature=np.ldexp(temperature, exponent), **s)
+        assert got.tolist() == want.tolist(), s.keys()

@@ -758,7 +758,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   if (tid < 256) s.pow[tid] = g_powers.d[tid];
   float T = temperature ? temperature[row] : 1.f;
-  if (T > 0.f) T = fmaxf(T, 2e-36f);  // 256 log2(e) / T stays finite
   const int k = top_k ? top_k[row] : 0;
   const float P = top_p ? top_p[row] : 1.f;
   const float mp = min_p ? min_p[row] : 0.f;
@@ -849,7 +848,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   Sampler<CL, RES> a = {s, RES ? x : src, maxima, smem, rank, begin, len, head, tid, lane, warp,
                    top, far, 369.3299304675746 / (double)T,
                M > 0.f && T < INFINITY ? -log((double)M) * (double)T : (double)INFINITY,
-                   range > 0.f ? (float)kBuckets / range : 0.f, far, INT_MAX, 0};
+                   range > 0.f ? fminf((float)kBuckets / range, FLT_MAX) : 0.f, far, INT_MAX, 0};
   if (k > 0 && k < vocab && a.template filter<false>(k, P, u, tokens + row)) return;
   if (P < 1.f && a.template filter<true>(k, P, u, tokens + row)) return;
   // The draw by sums, of every 128 neighbouring logits first.
@@ -866,8 +865,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   // logits after them.
   u64* sums = reinterpret_cast<u64*>(smem);
   const int parts = (a.n_quads() + 31) / 32 + 2;
-  // (min-p's distance with room for the roundings)
-  const float least = fmaxf(a.least, top - (float)a.reach_p * 1.00001f);
+  // (min-p's distance with room for the roundings, which are large among subnormals)
+  const float least =
+      fmaxf(a.least, __fsub_rd(top, __fmul_ru(__double2float_ru(a.reach_p), 1.00001f)));
   for (int it = 0; it < a.n_batches(); ++it) {
     const bool active = maxima[it * kThreads + tid] >= least;  // -inf past the last quad
     const int first = 1 + it * kQuads * kWarps + warp;
