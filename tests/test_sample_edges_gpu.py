@@ -83,3 +83,26 @@ def test_tiny_logits_and_temperatures(rows, exponent):
                 want[r], near = sample_row(x[r], u[r], temperature[r], **one)
         got = draw(scaled, u, temperature=np.ldexp(temperature, exponent), **s)
         assert got.tolist() == want.tolist(), s.keys()
+
+
+@pytest.mark.parametrize("rows", [1, 8, 70, 200])
+@pytest.mark.parametrize("temperature", [3e37, 1e38, np.inf])
+def test_logits_further_apart_than_the_type_reaches(rows, temperature):
+    """The row's range and 33 temperatures both pass the largest FP32 number; the cut lies
+    among the far logits."""
+    vocab = 70001
+    rng = np.random.default_rng(rows)
+    x = (rng.choice([-1, 1, 1, 1], (rows, vocab)) * rng.uniform(2e38, 3.3e38, (rows, vocab))).astype(np.float32)
+    t = np.full(rows, temperature)
+    for s in ({}, {"top_k": np.full(rows, vocab - 500)}, {"top_p": np.full(rows, 0.999)},
+              {"top_k": np.full(rows, 60000), "top_p": np.full(rows, 0.98)}):
+        # equal weights: the borders are multiples of one of them, and u lies between
+        u = ((rng.integers(0, 60000, rows) + 0.5) / 60000).astype(np.float32)
+        got = draw(x, u, temperature=t, **s)
+        for r in range(rows):
+            one = {k: (int if k == "top_k" else np.float32)(v[r]) for k, v in s.items()}
+            want, near = sample_row(x[r], u[r], np.float32(temperature), **one)
+            if near > vocab * 2.0 ** -43:
+                assert got[r] == want, (r, one, int(got[r]), want)
+            else:
+                assert 0 <= got[r] < vocab

@@ -843,8 +843,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   // `far` 22 T below it, where a weight is 3929 of 2^-44.
   const float far = fmaxf(fminf(__fsub_rd(top, __fmul_ru(kFar, T)), under), -FLT_MAX);
   // Buckets over the distances that have weight, or over the row's own range
-  // where that is narrower (and not a masked row's, whose least is -inf).
-  const float range = fminf(kFar * T, top - lo);
+  // where that is narrower (and not a masked row's, whose least is -inf).  Finite, so
+  // that the buckets of far logits have an end in every case.
+  const float range = fminf(fminf(kFar * T, top - lo), FLT_MAX);
   Sampler<CL, RES> a = {s, RES ? x : src, maxima, smem, rank, begin, len, head, tid, lane, warp,
                    top, far, 369.3299304675746 / (double)T,
                M > 0.f && T < INFINITY ? -log((double)M) * (double)T : (double)INFINITY,
