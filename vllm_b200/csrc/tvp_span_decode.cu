@@ -106,6 +106,7 @@ __global__ void __launch_bounds__(Shape<KVH, SHARED>::kThreads, Shape<KVH, SHARE
   extern __shared__ __align__(1024) unsigned char smem[];
   if (smem_addr(smem) & 1023u) {
     if (threadIdx.x == 0) record_error(p.err, TVP_DEVERR_SMEM_ALIGN);
+    if (!SHARED) asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cta::kBarsAt);
@@ -405,7 +406,11 @@ __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const Sp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool in_order = groups_in_order(p);
   const int at = blockIdx.x * kMergeWarps + warp, s = at / KVH, h = at % KVH;
-  if (!in_order || s >= p.batch) return;
+  if (!in_order || s >= p.batch) {
+    // Later work of the stream is behind the call's other launches through this wait.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   // What the call's inputs say, before the launches before this one are done.
   const RowSpan span = decode_span<true>(p, s, false);
   const int g = span.len > 0 ? group_of(p, s) : -1;

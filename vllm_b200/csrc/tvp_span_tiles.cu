@@ -164,6 +164,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t sbase = smem_addr(smem);
   if (sbase & 1023u) {
     if (threadIdx.x == 0) record_error(p.err, TVP_DEVERR_SMEM_ALIGN);
+    if (PREFIX) asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
