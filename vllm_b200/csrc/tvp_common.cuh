@@ -79,6 +79,13 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity)
   }
 }
 
+// True when `count` positions from `first` on lie on a block-table row.  In 64 bits: a
+// sum of 32-bit positions next to the largest would overflow, which the compiler
+// takes as never happening and drops the comparison that should see it.
+__device__ __forceinline__ bool positions_on_table(long long first, int count, int table_stride) {
+  return first >= 0 && first + count <= (long long)table_stride * kPage;
+}
+
 // mbar_wait_bounded that sleeps `ns` between its tests: a wait that polls takes
 // issue slots from the warps of its SM sub-partition that have work.
 __device__ __forceinline__ bool mbar_wait_sleeping(uint32_t bar, uint32_t parity, unsigned ns) {

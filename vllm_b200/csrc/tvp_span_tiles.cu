@@ -210,12 +210,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     tok0 = q_begin + tile * kTileRows;
     if (tok0 >= q_end) return;  // this sequence has fewer tiles
     count = min(kTileRows, q_end - tok0);
-    pos0 = __ldg(p.q_pos0 + s) + tile * kTileRows;  // position of the tile's token 0
-    pos_last = pos0 + count - 1;
-    if (pos0 < 0 || pos_last / kPage >= p.table_stride) {
+    const long long at0 = (long long)__ldg(p.q_pos0 + s) + tile * kTileRows;
+    if (!positions_on_table(at0, count, p.table_stride)) {
       if (threadIdx.x == 0) record_error(p.err, TVP_DEVERR_BAD_TOKEN);
       return;
     }
+    pos0 = (int)at0;  // position of the tile's token 0
+    pos_last = pos0 + count - 1;
     span = window_span(pos_last + 1, (long long)pos0 + 1 - p.window, p.sinks);
     v_begin = 0;
     v_end = span.pages;
