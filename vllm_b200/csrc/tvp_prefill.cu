@@ -139,12 +139,13 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   const int tok0 = q_begin + tile * kTcTokens;
   if (tok0 >= q_end) return;  // this sequence has fewer tiles
   const int count = min(kTcTokens, q_end - tok0);
-  const int pos0 = __ldg(p.q_pos0 + s) + tile * kTcTokens;  // position of the tile's token 0
-  const int pos_last = pos0 + count - 1;
-  if (pos0 < 0 || pos_last / kPage >= p.table_stride) {
+  const long long at0 = (long long)__ldg(p.q_pos0 + s) + tile * kTcTokens;
+  if (!positions_on_table(at0, count, p.table_stride)) {
     if (threadIdx.x == 0) record_error(p.err, TVP_DEVERR_BAD_TOKEN);
     return;
   }
+  const int pos0 = (int)at0;  // position of the tile's token 0
+  const int pos_last = pos0 + count - 1;
   const int last_page = pos_last / kPage;
   const int n_chunks = pos_last / kTcChunk + 1;
 
