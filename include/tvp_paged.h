@@ -402,6 +402,9 @@ int tvp_head_gather_destroy(tvp_head_gather* g);
  * counterparts in the reference, whose decode attends each row's whole
  * context on its own (src/model/paged_transformer.cu:85-94).  Pools, tables
  * and error bits are as above; kv_heads is 8, 4, 2 or 1, q_heads = 4 kv_heads.
+ * TVP_ERR_UNSUPPORTED where a row's positions, or the pages that a decode
+ * batch may see (batch times table_stride, or times a window's and its sinks'
+ * pages), pass 32 bits.
  * Scores and softmax statistics are FP32, probabilities BF16 into an FP32
  * P.V, outputs BF16.
  * ======================================================================= */

@@ -22,6 +22,11 @@ int resolve_span_ctas(int num_ctas, int* out) {
 
 constexpr int kMaxStride = INT_MAX / kPage;  // token positions are 32-bit
 
+// The kernels add up the pages that the rows see in 32 bits.
+bool pages_countable(int batch, long long pages_per_row) {
+  return batch * pages_per_row <= INT_MAX;
+}
+
 bool span_heads_supported(int kv_heads) {
   return kv_heads == 1 || kv_heads == 2 || kv_heads == 4 || kv_heads == kMaxKvHeads;
 }
@@ -108,6 +113,9 @@ int tvp_paged_window_decode_attention(const tvp_bf16* q, const tvp_bf16* k_pool,
   if (rc != TVP_OK) return rc;
   if (window < 1 || sinks < 0) return TVP_ERR_INVALID_ARGUMENT;
   if (table_stride > kMaxStride) return TVP_ERR_UNSUPPORTED;
+  // (a window that starts inside a page sees one page more)
+  const long long seen = ((long long)window + kPage - 1) / kPage + ((long long)sinks + kPage - 1) / kPage + 1;
+  if (!pages_countable(batch, seen < table_stride ? seen : table_stride)) return TVP_ERR_UNSUPPORTED;
   int ctas = 0;
   if ((rc = resolve_span_ctas(num_ctas, &ctas)) != TVP_OK) return rc;
   const SpanWorkspace w = span_workspace(batch, 0, kv_heads, ctas);
@@ -138,7 +146,8 @@ int tvp_paged_shared_prefix_decode_attention(
   if (groups < 0 || groups > 65535 || prefix_stride < 0 || !aligned(q, 16) ||
       (groups > 0 && (!d_prefix_tables || !d_prefix_pages || !d_group_rows || prefix_stride < 1)))
     return TVP_ERR_INVALID_ARGUMENT;
-  if (table_stride > kMaxStride || prefix_stride > kMaxStride) return TVP_ERR_UNSUPPORTED;
+  if (table_stride > kMaxStride || prefix_stride > kMaxStride || !pages_countable(batch, table_stride))
+    return TVP_ERR_UNSUPPORTED;
   int ctas = 0;
   if ((rc = resolve_span_ctas(num_ctas, &ctas)) != TVP_OK) return rc;
   const SpanWorkspace w = span_workspace(batch, groups, kv_heads, ctas);
