@@ -453,7 +453,8 @@ int tvp_paged_window_decode_attention(const tvp_bf16* q, const tvp_bf16* k_pool,
  * its first d_seq_lens[b] tokens.  A row of length 0 gets zeros; one shorter
  * than its prefix gets zeros and TVP_DEVERR_BAD_LENGTH.  Group rows that are
  * out of order set TVP_DEVERR_BAD_PLAN and nothing is written.  groups = 0 is
- * plain decode attention.  Three launches on `stream`.
+ * plain decode attention.  Three launches on `stream`, four with more than 192
+ * groups.
  */
 int tvp_paged_shared_prefix_decode_attention(
     const tvp_bf16* q, const tvp_bf16* k_pool, const tvp_bf16* v_pool, int num_pages,

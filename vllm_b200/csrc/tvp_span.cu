@@ -36,7 +36,7 @@ struct SpanWorkspace {
   int max_pieces;
 };
 
-// counters[1024][8] | row_ranges[batch] | group_pieces[groups] | partials | pieces.
+// counters[1024][8] | row_ranges[batch] | group_pieces[groups + 1] | partials | pieces.
 // The counters' place and size are the same for every call.  Pieces: one
 // per CTA, or per tile of 32 rows and KV head where those are more.
 SpanWorkspace span_workspace(int batch, int groups, int kv_heads, int num_ctas) {
@@ -44,7 +44,7 @@ SpanWorkspace span_workspace(int batch, int groups, int kv_heads, int num_ctas) 
   SpanWorkspace w = {};
   w.row_ranges = (size_t)kMaxSpanCtas * kMaxKvHeads * 4;
   w.group_pieces = w.row_ranges + (groups > 0 ? align((size_t)batch * sizeof(int2)) : 0);
-  w.partials = align(w.group_pieces + (size_t)groups * sizeof(int2));
+  w.partials = align(w.group_pieces + (groups > 0 ? (size_t)groups + 1 : 0) * sizeof(int2));
   const size_t slots = groups > 0 ? (size_t)batch + num_ctas : (size_t)2 * num_ctas;
   w.pieces = align(w.partials + slots * kv_heads * kPartialFloats * 4);
   if (groups > 0) {
@@ -166,6 +166,7 @@ int tvp_paged_shared_prefix_decode_attention(
   fill_workspace(d_workspace, w, ctas, &p);
   const long long rows = (long long)num_layers * num_pages * kPage;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (groups > kWarpGroups && (rc = map_cuda(launch_prefix_plan(p, st))) != TVP_OK) return rc;
   if ((rc = map_cuda(launch_span_decode(p, groups > 0, rows, ctas, st))) != TVP_OK || groups == 0)
     return rc;
   if ((rc = map_cuda(launch_prefix_tiles(p, rows, w.max_pieces, st))) != TVP_OK) return rc;

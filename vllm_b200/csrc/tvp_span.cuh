@@ -10,6 +10,11 @@ namespace tvp {
 constexpr int kMaxSpanCtas = 1024;
 constexpr int kTileRows = 32;   // batch rows (or query tokens) of one MMA tile
 constexpr int kChunkPages = 4;  // pages per key chunk of a tile
+// Prefix groups up to which each CTA works the pieces out by itself; a plan saves
+// that and costs a launch.  By itself / planned, us, groups of two rows behind 128
+// tokens: of 8 heads 150 52 / 52, 192 67 / 65, 1000 763 / 275; of one head 150 20 / 24,
+// 192 23 / 28, 1000 122 / 71.
+constexpr int kWarpGroups = 192;
 // One piece of a shared prefix: per row of the tile an (m, l, O) partial.
 constexpr size_t kPieceFloats = (size_t)kTileRows * kPartialFloats;
 
@@ -37,7 +42,8 @@ struct SpanParams {
                        // [row + range][kv_heads]
   // rows with prefixes
   int2* row_ranges;    // [batch]: first and last range of a row's own pages
-  int2* group_pieces;  // [groups]: first piece, pieces per (tile, KV head)
+  int2* group_pieces;  // [groups + 1]: first piece, pieces per (tile, KV head); with a plan the
+                       // last entry says whether the group rows are in order
   float* pieces;       // [piece][row of the tile] partials of the shared prefixes
   int piece_target;    // pieces to aim at
 };
@@ -128,6 +134,12 @@ __device__ __forceinline__ bool groups_in_order(const SpanParams& p) {
   return !__syncthreads_or(bad);
 }
 
+// The same, read from the plan where there is one.
+__device__ __forceinline__ bool groups_usable(const SpanParams& p) {
+  return p.groups <= kWarpGroups ? groups_in_order(p) : __ldg(&p.group_pieces[p.groups].x) != 0;
+}
+
+cudaError_t launch_prefix_plan(const SpanParams& p, cudaStream_t stream);
 cudaError_t launch_span_decode(const SpanParams& p, bool shared, long long pool_rows, int num_ctas,
                                cudaStream_t stream);
 cudaError_t launch_prefix_tiles(const SpanParams& p, long long pool_rows, int max_pieces,

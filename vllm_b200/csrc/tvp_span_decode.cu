@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(Shape<KVH, SHARED>::kThreads, Shape<KVH, SHARE
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // The tile kernel may start beside this one.
   if (SHARED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (SHARED && !groups_in_order(p)) {
+  if (SHARED && !groups_usable(p)) {
     if (tid == 0 && blockIdx.x == 0) record_error(p.err, TVP_DEVERR_BAD_PLAN);
     return;
   }
@@ -404,7 +404,7 @@ constexpr int kMergeWarps = 4;  // of a block; 8: 256 rows 79.0 us instead of 78
 template <int KVH>
 __global__ void __launch_bounds__(kMergeWarps * 32) prefix_merge_kernel(const SpanParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool in_order = groups_in_order(p);
+  const bool in_order = groups_usable(p);
   const int at = blockIdx.x * kMergeWarps + warp, s = at / KVH, h = at % KVH;
   if (!in_order || s >= p.batch) {
     // Later work of the stream is behind the call's other launches through this wait.

@@ -9,7 +9,8 @@
 //     pieces per SM, one after the other, took 26.7 us instead of 18.2 for 8 rows
 //     behind 8192 tokens, 78 instead of 75 for 256), so a few long prefixes and
 //     many short ones both fill the GPU once; every CTA works this out from the
-//     group sizes, a search of some ten steps by one warp.
+//     group sizes, a search of some ten steps by one warp, or, of more groups than
+//     kWarpGroups, reads it from a plan.
 //   * window: the tokens are a tile of a sequence's queries, the pages the ones
 //     that some query of the tile sees; the CTA writes the output rows.
 //
@@ -82,9 +83,41 @@ __device__ __forceinline__ int2 group_work(const SpanParams& p, int g) {
   return make_int2(chunks > 0 ? (rows + kTileRows - 1) / kTileRows * p.kv_heads : 0, chunks);
 }
 
-// Piece `index` of the prefixes, by one warp; group < 0 past the last.  The
-// first block also leaves every group's first piece and count of pieces per
-// stream for the merge kernel.
+// The shortest length of a piece, in chunks, whose pieces fit piece_target, between
+// the even share and one piece per stream; count(n) is the number of pieces of n
+// chunks.
+template <typename Count>
+__device__ __forceinline__ int piece_length(const SpanParams& p, long long streams, long long work,
+                                            int most, Count count) {
+  most = max(most, kMinChunks);
+  if (streams >= p.piece_target) return most;
+  const long long even = (work + p.piece_target - 1) / p.piece_target;
+  int lo = (int)(even > kMinChunks ? even : kMinChunks), hi = max(most, lo);
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (count(mid) <= p.piece_target)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo;
+}
+
+// Piece `at` of group g, whose streams have `splits` pieces each.
+__device__ __forceinline__ Piece piece_of(const SpanParams& p, int g, int chunks, int splits, int at) {
+  const int stream = at / splits, j = at % splits;
+  Piece out;
+  out.group = g;
+  out.tile = stream / p.kv_heads;
+  out.head = stream % p.kv_heads;
+  out.first = (int)((long long)chunks * j / splits) * kChunkPages;
+  out.last = min(shared_pages(p, g, false), (int)((long long)chunks * (j + 1) / splits) * kChunkPages);
+  return out;
+}
+
+// Piece `index` of the prefixes of up to kWarpGroups groups, by one warp; group < 0
+// past the last.  The first block also leaves every group's first piece and count of
+// pieces per stream for the merge kernel.
 __device__ __forceinline__ Piece find_piece(const SpanParams& p, int index, int lane, bool publish) {
   auto sum = [](long long v) {
 #pragma unroll
@@ -102,29 +135,20 @@ __device__ __forceinline__ Piece find_piece(const SpanParams& p, int index, int 
   streams = sum(streams);
   work = sum(work);
   most = __reduce_max_sync(0xffffffffu, most);
-  const long long limit = streams > p.piece_target ? streams : p.piece_target;
-  // the shortest length whose pieces fit the limit, between the even share and
-  // one piece per stream
-  long long at_least = (work + limit - 1) / limit;
-  int lo = (int)(at_least > kMinChunks ? at_least : kMinChunks), hi = max(most, lo);
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    long long n = 0;
+  const int length = piece_length(p, streams, work, most, [&](int n) {
+    long long pieces = 0;
     for (int g = lane; g < p.groups; g += 32) {
       const int2 w = group_work(p, g);
-      n += (long long)w.x * ((w.y + mid - 1) / mid);
+      pieces += (long long)w.x * ((w.y + n - 1) / n);
     }
-    if (sum(n) <= limit)
-      hi = mid;
-    else
-      lo = mid + 1;
-  }
+    return sum(pieces);
+  });
   Piece out = {-1, 0, 0, 0, 0};
   int before = 0;
   for (int base = 0; base < p.groups; base += 32) {
     const int g = base + lane;
     const int2 w = g < p.groups ? group_work(p, g) : make_int2(0, 0);
-    const int splits = (w.y + lo - 1) / lo;
+    const int splits = (w.y + length - 1) / length;
     const int n = w.x * splits;
     int inc = n;
 #pragma unroll
@@ -134,25 +158,103 @@ __device__ __forceinline__ Piece find_piece(const SpanParams& p, int index, int 
     }
     const int first = before + inc - n;
     if (publish && g < p.groups) p.group_pieces[g] = make_int2(first, n > 0 ? splits : 0);
-    const bool here = index >= first && index < first + n;
-    const uint32_t who = __ballot_sync(0xffffffffu, here);
+    const uint32_t who = __ballot_sync(0xffffffffu, index >= first && index < first + n);
     if (who) {
       const int src = __ffs(who) - 1;
-      const int at = index - __shfl_sync(0xffffffffu, first, src);
-      const int k = __shfl_sync(0xffffffffu, splits, src);
-      const int chunks = __shfl_sync(0xffffffffu, w.y, src);
-      const int stream = at / k, j = at % k;
-      out.group = base + src;
-      out.tile = stream / p.kv_heads;
-      out.head = stream % p.kv_heads;
-      const int pages = shared_pages(p, out.group, false);
-      out.first = (int)((long long)chunks * j / k) * kChunkPages;
-      out.last = min(pages, (int)((long long)chunks * (j + 1) / k) * kChunkPages);
+      out = piece_of(p, base + src, __shfl_sync(0xffffffffu, w.y, src), __shfl_sync(0xffffffffu, splits, src),
+                     index - __shfl_sync(0xffffffffu, first, src));
       if (!publish) return out;
     }
     before += __shfl_sync(0xffffffffu, inc, 31);
   }
   return out;
+}
+
+// The same for more groups, in two steps: one block works out every group's first
+// piece, a launch before the others, and a CTA finds its group by bisection, so that
+// the cost grows with the groups and not with their square.
+constexpr int kPlanThreads = 1024;
+
+__global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(const SpanParams p) {
+  __shared__ long long sums[kPlanThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // Sum over the block, in every thread; two barriers.
+  auto sum = [&](long long v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) sums[warp] = v;
+    __syncthreads();
+    v = sums[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    return v;
+  };
+  const bool in_order = groups_in_order(p);
+  if (tid == 0) p.group_pieces[p.groups] = make_int2(in_order, 0);
+  if (!in_order) return;  // the decode kernel reports it
+  long long streams = 0, work = 0;
+  int most = 1;
+  for (int g = tid; g < p.groups; g += kPlanThreads) {
+    shared_pages(p, g, true);
+    const int2 w = group_work(p, g);
+    streams += w.x;
+    work += (long long)w.x * w.y;
+    if (w.x > 0) most = max(most, w.y);
+  }
+  streams = sum(streams);
+  work = sum(work);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) sums[warp] = most;
+  __syncthreads();
+  most = __reduce_max_sync(0xffffffffu, (int)sums[lane]);
+  __syncthreads();
+  const int length = piece_length(p, streams, work, most, [&](int n) {
+    long long pieces = 0;
+    for (int g = tid; g < p.groups; g += kPlanThreads) {
+      const int2 w = group_work(p, g);
+      pieces += (long long)w.x * ((w.y + n - 1) / n);
+    }
+    return sum(pieces);
+  });
+  int before = 0;
+  for (int base = 0; base < p.groups; base += kPlanThreads) {
+    const int g = base + tid;
+    const int2 w = g < p.groups ? group_work(p, g) : make_int2(0, 0);
+    const int splits = (w.y + length - 1) / length, n = w.x * splits;
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) sums[warp] = inc;
+    __syncthreads();
+    int lower = 0, total = 0;
+    for (int i = 0; i < kPlanThreads / 32; ++i) {
+      if (i < warp) lower += (int)sums[i];
+      total += (int)sums[i];
+    }
+    __syncthreads();
+    if (g < p.groups) p.group_pieces[g] = make_int2(before + lower + inc - n, n > 0 ? splits : 0);
+    before += total;
+  }
+}
+
+// Piece `index` by the plan.
+__device__ __forceinline__ Piece planned_piece(const SpanParams& p, int index) {
+  int lo = 0, hi = p.groups;  // first piece of group lo <= index < that of group hi
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(&p.group_pieces[mid].x) <= index)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const int2 in = __ldg(p.group_pieces + lo);
+  const int2 w = group_work(p, lo);
+  if (in.y == 0 || index - in.x >= w.x * in.y) return {-1, 0, 0, 0, 0};
+  return piece_of(p, lo, w.y, in.y, index - in.x);
 }
 
 template <bool PREFIX>
@@ -182,11 +284,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       asm volatile("griddepcontrol.wait;" ::: "memory");
       return;
     }
-    if (!groups_in_order(p)) return;  // the decode kernel reports it
+    if (!groups_usable(p)) return;  // the decode kernel reports it
     Piece* shared_piece = reinterpret_cast<Piece*>(smem + kOffPlan);
     if (warp == 0) {
-      const bool publish = blockIdx.x == 0;
-      const Piece mine = find_piece(p, blockIdx.x, lane, publish);
+      const bool publish = p.groups <= kWarpGroups && blockIdx.x == 0;
+      const Piece mine = p.groups <= kWarpGroups ? find_piece(p, blockIdx.x, lane, publish)
+                                                 : planned_piece(p, blockIdx.x);
       if (lane == 0) *shared_piece = mine;
       if (publish)
         for (int i = lane; i < p.groups; i += 32) shared_pages(p, i, true);
@@ -647,6 +750,11 @@ cudaError_t launch_tiles(const SpanParams& p, long long pool_rows, dim3 grid, cu
 }
 
 }  // namespace
+
+cudaError_t launch_prefix_plan(const SpanParams& p, cudaStream_t stream) {
+  prefix_plan_kernel<<<1, kPlanThreads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
 
 cudaError_t launch_prefix_tiles(const SpanParams& p, long long pool_rows, int max_pieces,
                                 cudaStream_t stream) {
