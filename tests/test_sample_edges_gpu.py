@@ -106,3 +106,17 @@ def test_logits_further_apart_than_the_type_reaches(rows, temperature):
                 assert got[r] == want, (r, one, int(got[r]), want)
             else:
                 assert 0 <= got[r] < vocab
+
+
+@pytest.mark.parametrize("rows", [63, 64, 95, 96, 191, 192])
+@pytest.mark.parametrize("vocab", [32768, 32769])
+def test_rows_agree_on_both_sides_of_every_size(rows, vocab):
+    """A row's token is the same in the form that its batch takes and in that of a few rows."""
+    rng = np.random.default_rng(rows)
+    x = np.round(rng.standard_normal((rows, vocab)) * 3, 1).astype(np.float32)  # with equal logits
+    u = rng.random(rows)
+    s = {"temperature": rng.choice([0.5, 1.0], rows), "top_k": rng.choice([0, 40, 900], rows),
+         "top_p": rng.choice([0.5, 0.9, 1.0], rows), "min_p": rng.choice([0.0, 0.05], rows)}
+    few = np.concatenate([draw(x[i:i + 30], u[i:i + 30], **{k: v[i:i + 30] for k, v in s.items()})
+                          for i in range(0, rows, 30)])
+    assert np.array_equal(draw(x, u, **s), few)

@@ -59,6 +59,12 @@ constexpr int kBlocks = kBuckets / 32;  // two per lane of a warp
 // streaming: 32 rows 32 / 46 / 76, 64 rows 50 / 51 / 77, 96 rows 69 / 60 / 71,
 // 256 rows 157 / 115 / 117; of top-k 50: 32 rows 14 / 14 / 17, 64 rows
 // 27 / 16 / 17, 256 rows 105 / 65 / 47.
+// Shorter rows (kShortVocab) are mostly barriers, and go to 2 CTAs from kStreamShort
+// rows on.  Mixed settings / top-k 50, 4 CTAs against 2: of 8000 logits 64 rows
+// 23.5 / 13.5 against 21.4 / 12.3, 96 rows 30.2 / 24.1 against 22.3 / 14.3, 191 rows
+// 45.3 / 36.2 against 31.7 / 24.6; of 32000 80 rows 27.1 / 23.6 against 30.3 / 14.9, 96
+// rows 31.7 / 25.1 against 32.6 / 14.9, 191 rows 49.3 / 37.4 against 35.4 / 26.2; of
+// 50257 96 rows 33.8 / 27.4 against 45.2 / 16.7.
 // A few rows of a large vocabulary: 16 CTAs.  One row, top-p 0.9, 8 CTAs / 16: of
 // 300000 logits 51 / 37 us, of 128256 25 / 22, of 50257 20.5 / 20.2, of 1000
 // 9.7 / 10.3 (a larger cluster's barriers take longer); 8 rows of 128256 27.9 / 27.4
@@ -69,6 +75,8 @@ constexpr int kWideVocab = 65536;
 static_assert(kBlocks == 64 && kBuckets / kWide % 32 == 0, "border() deals them out so");
 constexpr int kStreamRows = 64;
 constexpr int kStreamMany = 192;
+constexpr int kStreamShort = 96;
+constexpr int kShortVocab = 32768;
 constexpr int kList = 512;  // logits of a bucket that CTA 0 takes in
 // Logits at or above the cut that CTA 0 finishes by itself, each compared with
 // each by two threads or more per logit.  Top-k 200 that way: one row 14.4 us, 256
@@ -1033,8 +1041,9 @@ extern "C" int tvp_sample_tokens(const float* d_logits, int rows, int vocab, lon
   cudaError_t e = cudaErrorNotSupported;
   if (rows <= kWideRows && vocab >= kWideVocab) e = run(launch_sampler<kWide, true>);
   if (e == cudaErrorNotSupported)
-    e = run(rows < kStreamRows   ? launch_sampler<kCluster, true>
-            : rows < kStreamMany ? launch_sampler<4, false>
-                                 : launch_sampler<2, false>);
+    e = run(rows < kStreamRows ? launch_sampler<kCluster, true>
+            : rows < (vocab > kShortVocab ? kStreamMany : kStreamShort)
+                ? launch_sampler<4, false>
+                : launch_sampler<2, false>);
   return e == cudaSuccess ? TVP_OK : TVP_ERR_RUNTIME;
 }
