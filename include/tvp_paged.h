@@ -406,7 +406,11 @@ int tvp_head_gather_destroy(tvp_head_gather* g);
  * batch may see (batch times table_stride, or times a window's and its sinks'
  * pages), pass 32 bits.
  * Scores and softmax statistics are FP32, probabilities BF16 into an FP32
- * P.V, outputs BF16.
+ * P.V, outputs BF16.  Keys keep the positions that they were rotated for when
+ * they were appended, behind a window too: nothing is renumbered.  An entry
+ * read that is no page sets TVP_DEVERR_BAD_PAGE; its 16 tokens are left out of
+ * the row (window decode, a row's own pages) or count as keys and values of
+ * zero (window prefill, shared prefixes).
  * ======================================================================= */
 
 /*
@@ -445,10 +449,10 @@ int tvp_paged_window_decode_attention(const tvp_bf16* q, const tvp_bf16* k_pool,
  * K7 — decode attention of a batch whose rows share long prefixes, each prefix
  * read once per 32 rows of its group instead of once per row.
  * Group g holds the rows [d_group_rows[g], d_group_rows[g + 1]) (non-decreasing,
- * within 0..batch; rows outside every group share nothing).  The first
- * 16 * d_prefix_pages[g] tokens of each of its rows are the pages
- * d_prefix_tables[g * prefix_stride ..]; a row's later tokens are on the pages
- * of its own block-table row, which stays indexed by position (entry
+ * within 0..batch; rows outside every group share nothing; 65,535 groups at
+ * most).  The first 16 * d_prefix_pages[g] tokens of each of its rows are the
+ * pages d_prefix_tables[g * prefix_stride ..]; a row's later tokens are on the
+ * pages of its own block-table row, which stays indexed by position (entry
  * position / 16; the entries of the shared pages are not read).  Row b attends
  * its first d_seq_lens[b] tokens.  A row of length 0 gets zeros; one shorter
  * than its prefix gets zeros and TVP_DEVERR_BAD_LENGTH.  Group rows that are
@@ -468,7 +472,9 @@ int tvp_paged_shared_prefix_decode_attention(
  * K8 — causal prefill attention with a sliding window and attention sinks,
  * over the pages: tvp_paged_prefill_attention's queries and layout, where the
  * query at position p sees key j <= p when j > p - window or j < sinks.  Pages
- * that no query of a 32-token tile sees are not read by that tile.
+ * that no query of a 32-token tile sees are not read by that tile.  A hidden
+ * value counts as 0 times itself, so an infinity or NaN that one query of a tile
+ * sees may reach the others.
  */
 int tvp_paged_window_prefill_attention(const tvp_bf16* q, const tvp_bf16* k_pool,
                                        const tvp_bf16* v_pool, int num_pages, int num_layers,
@@ -498,7 +504,7 @@ int tvp_paged_window_prefill_attention(const tvp_bf16* q, const tvp_bf16* k_pool
  * as 64-bit integers of 2^-44 of the largest weight, so the result does not
  * depend on the order of the sums.  Unlike tvp_greedy_argmax, logits are not
  * rounded to BF16.  d_logits: [rows][row_stride], row_stride >= vocab; vocab at
- * most TVP_SAMPLE_MAX_VOCAB.  No workspace.
+ * most TVP_SAMPLE_MAX_VOCAB, 65,535 rows at most.  No workspace.
  */
 #define TVP_SAMPLE_MAX_VOCAB 327680
 int tvp_sample_tokens(const float* d_logits, int rows, int vocab, long long row_stride,

@@ -25,13 +25,14 @@
 // the 128 at the point.  For a small top-k the histogram is one of the largest
 // logits of every 32, which costs no pass over the row.
 //
-// What bounds it, at rows of 128256 logits: one row 8.1 us without filters, 10
+// What bounds it, at rows of 128256 logits: one row 8.3 us without filters, 10.5
 // with top-k 50, 22 with top-p 0.9 (launch, a chain of cluster barriers of about
 // 0.5 us and reads of other CTAs' shared memory, and passes of one row over 16
-// SMs); 256 rows without filters 68 us (131 MB: 1.9 TB/s; the weights' FP64
+// SMs; the 16-CTA form also spills 184 bytes a thread at its 64 registers);
+// 256 rows without filters 69 us (131 MB: 1.9 TB/s; the weights' FP64
 // arithmetic takes 50 of them), with top-k 50 45 us (2.9 TB/s: the first pass
 // streams at the HBM rate, the chain behind it is the same as for one row), with
-// top-p 0.9 199 us (a weight into a shared-memory histogram, two 32-bit atomics,
+// top-p 0.9 200 us (a weight into a shared-memory histogram, two 32-bit atomics,
 // for each logit with one).
 #include <cfloat>
 #include <climits>

@@ -211,9 +211,8 @@ __global__ void __launch_bounds__(Shape<KVH, SHARED>::kThreads, Shape<KVH, SHARE
       span = decode_span<SHARED>(p, s, false);
       walk();
     }
-    // Launched as a programmatic dependent launch: the kernel before may still
-    // run.  It writes pages and q, never lengths or tables, so the walk starts
-    // now and the wait comes before the first copy.  (SHARED starts after it.)
+    // The kernel before is done (the wait at the top; SHARED starts after it): what
+    // it wrote to the pages is ordered before this warp's copies.
     if (!SHARED) asm volatile("fence.proxy.async.global;" ::: "memory");
     const int n_stages = (n + PS - 1) / PS;
     int stage = 0, issued = 0;
