@@ -6,6 +6,7 @@ import torch
 import span_cases as S
 import test_shared_prefix_gpu as P
 import test_window_attention_gpu as T
+from gpu_util import dev_bf16, dev_i32, host_bf16
 from vllm_b200 import _native as N
 from vllm_b200 import ops
 from workloads import bf16_to_f32
@@ -86,3 +87,48 @@ def test_one_workspace_for_few_groups_and_many():
         got, err = P.run(case, workspace=ws)
         assert err == 0
         S.check(got, case)
+
+
+def test_many_groups_captured_and_replayed_with_other_groups():
+    """A captured call reads the group rows, prefixes and lengths of each replay, its plan among them."""
+    rng = np.random.default_rng(12)
+    cases = []
+    for seed in (1, 2, 3):
+        groups = [(1, int(p)) for p in rng.integers(0, 6, 200)]
+        order = rng.permutation(200)
+        cases.append(S.SpanCase(400 + seed, P.rows(rng, [groups[i] for i in order], 50),
+                                groups=[groups[i] for i in order], kv_heads=1))
+    pages, stride = max(c.num_pages for c in cases), max(c.tables.shape[1] for c in cases)
+    pstride = max(c.prefix_tables.shape[1] for c in cases)
+
+    def inputs(c):
+        def wide(a, shape, fill):
+            out = np.full(shape, fill, a.dtype)
+            out[tuple(slice(n) for n in a.shape)] = a
+            return out
+        pool = (1, pages, 16, 64)
+        return [dev_bf16(c.q), dev_bf16(wide(c.k_pool, pool, 0x7FC0)), dev_bf16(wide(c.v_pool, pool, 0x7FC0)),
+                dev_i32(wide(c.tables, (200, stride), -1)), dev_i32(c.lens),
+                dev_i32(wide(c.prefix_tables, (200, pstride), -1)), dev_i32(c.prefix_pages), dev_i32(c.group_rows)]
+    args = inputs(cases[0])
+    ws, err, out = ops.SpanWorkspace(200, "cuda", kv_heads=1, max_groups=200), ops.new_error_word("cuda"), \
+        torch.empty_like(args[0])
+
+    def call():
+        ops.paged_shared_prefix_decode_attention(args[0], args[1], args[2], 0, *args[3:], ws, out=out, error=err)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        call()
+    for case in cases + cases[:1]:
+        for to, new in zip(args, inputs(case)):
+            to.copy_(new)
+        out.fill_(9)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(err.item()) == 0
+        S.check(host_bf16(out), case)
