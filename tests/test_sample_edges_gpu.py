@@ -120,3 +120,19 @@ def test_rows_agree_on_both_sides_of_every_size(rows, vocab):
     few = np.concatenate([draw(x[i:i + 30], u[i:i + 30], **{k: v[i:i + 30] for k, v in s.items()})
                           for i in range(0, rows, 30)])
     assert np.array_equal(draw(x, u, **s), few)
+
+
+def test_rows_behind_four_gigabytes():
+    """Rows that start past 2^32 bytes and 2^31 logits of a tensor give what they give alone."""
+    rows, vocab = 17000, 128256
+    assert rows * vocab > 1 << 31
+    x = torch.zeros((rows, vocab), device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    some = [0, 8371, 8372, 16743, 16744, 16999]
+    for r in some:
+        x[r] = torch.randn(vocab, generator=gen, device="cuda") * 2.5
+    u = torch.rand(rows, generator=gen, device="cuda")
+    k = torch.full((rows,), 40, dtype=torch.int32, device="cuda")
+    got = ops.sample_tokens(x, u, top_k=k)
+    alone = [int(ops.sample_tokens(x[r:r + 1].clone(), u[r:r + 1].clone(), top_k=k[:1])) for r in some]
+    assert got[some].tolist() == alone

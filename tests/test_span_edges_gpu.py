@@ -132,3 +132,38 @@ def test_many_groups_captured_and_replayed_with_other_groups():
         torch.cuda.synchronize()
         assert int(err.item()) == 0
         S.check(host_bf16(out), case)
+
+
+@pytest.mark.parametrize("form", ["decode", "prefill", "shared"])
+def test_pages_behind_four_gigabytes(form):
+    """The same pages, in a small pool and at the end of one of 4.7 GB (second of two layers)."""
+    if form == "shared":
+        case = S.SpanCase(71, [100, 64, 300, 17], groups=[(3, 4)])
+    else:
+        case = S.SpanCase(72, [300, 17, 90], window=70, sinks=5,
+                          q_counts=None if form == "decode" else [40, 17, 3])
+    pages = 144_000
+    pools = []
+    for bits in (case.k_pool, case.v_pool):
+        pool = torch.empty((2, pages, 16, 512), dtype=torch.bfloat16, device="cuda")
+        pool[1, pages - case.num_pages:].copy_(dev_bf16(bits)[0])
+        pools.append(pool)
+    assert pools[0].numel() * 2 > 1 << 32
+
+    def moved(table):
+        return dev_i32(np.where(table < 0, table, table + pages - case.num_pages))
+    q, err = dev_bf16(case.q), ops.new_error_word("cuda")
+    ws = ops.SpanWorkspace(len(case.lens), "cuda", max_groups=1)
+    if form == "decode":
+        out = ops.paged_window_decode_attention(q, *pools, 1, moved(case.tables), dev_i32(case.lens), case.window, ws,
+                                                sinks=case.sinks, error=err)
+    elif form == "prefill":
+        out = ops.paged_window_prefill_attention(q, *pools, 1, moved(case.tables), dev_i32(case.cu_q),
+                                                 dev_i32(case.q_pos0), 40, case.window, sinks=case.sinks, error=err)
+    else:
+        out = ops.paged_shared_prefix_decode_attention(
+            q, *pools, 1, moved(case.tables), dev_i32(case.lens), moved(case.prefix_tables),
+            dev_i32(case.prefix_pages), dev_i32(case.group_rows), ws, error=err)
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0
+    S.check(host_bf16(out), case)
